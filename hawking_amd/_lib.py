@@ -23,6 +23,7 @@ HK_E_NOMEM = 7
 HK_Q4, HK_BIN, HK_MIXED, HK_F32, HK_Q8, HK_U3, HK_BIN_RICE = 0, 1, 2, 3, 4, 5, 6
 HK_ROUTER_SOFTMAX, HK_ROUTER_NOAUX_TC = 0, 1
 HK_STACK_PER_LAYER, HK_STACK_PERSISTENT = 0, 1
+HK_T_F32, HK_T_BF16, HK_T_F16 = 0, 1, 2
 
 STATUS_NAMES = {
     HK_OK: "HK_OK", HK_E_INVALID_ARG: "HK_E_INVALID_ARG", HK_E_GEOMETRY: "HK_E_GEOMETRY",
@@ -88,6 +89,13 @@ class Moe15LayerSrc(C.Structure):
         ("shared_up", _p), ("shared_down", _p), ("gate", _p), ("up", _p), ("down_left", _p), ("down_right", _p),
     ]
 
+
+class RowsSrc(C.Structure):
+    """hk_rows: n rows in device memory, `stride` elements apart."""
+    _fields_ = [("data", _p), ("type", _i32), ("n", _u32), ("stride", _sz)]
+
+
+_rows = C.POINTER(RowsSrc)
 
 # name -> (restype, argtypes)
 PROTOTYPES = {
@@ -169,6 +177,17 @@ PROTOTYPES = {
     "hk_moe15_layer_free": (C.c_int, [_p, _p]),
     "hk_moe15_decode_layer": (C.c_int, [_p, _p, _p, _p, _p, _p, _p]),
     "hk_moe15_decode_stack": (C.c_int, [_p, _p, _u32, _p, _p, _p, _p, _p]),
+    "hk_group_rows_workspace": (_sz, [_u32, _u32]),
+    "hk_group_rows": (C.c_int, [_p, _p, _u32, _u32, _p, _p, _p, _p, _sz, _p]),
+    "hk_gemm_grouped_workspace": (_sz, [_p, _u32, _i32, _u32, _i32]),
+    "hk_gemm_grouped": (C.c_int, [_p, _p, _rows, _p, _u32, _p, _rows, _p, _sz, _p]),
+    "hk_gemm_grouped_swiglu": (C.c_int, [_p, _p, _p, _rows, _p, _u32, _p, _rows, _p, _sz, _p]),
+    "hk_combine_rows": (C.c_int, [_p, _rows, _p, _p, _u32, _u32, _rows, _rows, _p]),
+    "hk_lora_bank_create": (C.c_int, [_p, _p, _u32, _u32, C.POINTER(_p)]),
+    "hk_lora_bank_free": (C.c_int, [_p, _p]),
+    "hk_lora_bank_set": (C.c_int, [_p, _p, _u32, _u32, _p, _p, _i32, C.c_float, _p]),
+    "hk_gemm_lora_workspace": (_sz, [_p, _u32, _i32, _i32]),
+    "hk_gemm_lora": (C.c_int, [_p, _p, _p, _rows, _p, _p, _rows, _p, _sz, _p]),
 }
 
 _lib: C.CDLL | None = None

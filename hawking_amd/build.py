@@ -33,7 +33,8 @@ CFLAGS = [
 ]
 SOURCES = ["hk_api.cpp", "hk_gemv2.hip", "hk_repack.hip", "hk_pack.hip", "hk_router.hip", "hk_moe.hip",
            "hk_moe_batch.hip", "hk_rice.hip", "hk_head.hip", "hk_container.cpp", "hk_parse.cpp", "hk_moe15.hip",
-           "hk_moe_stack.hip", "hk_control.hip"]
+           "hk_moe_stack.hip", "hk_control.hip", "hk_rows_mixed.hip", "hk_rows_u3.hip", "hk_rows_q8.hip",
+           "hk_rows_q4.hip", "hk_rows_bin.hip", "hk_rows.hip", "hk_group.hip", "hk_lora.hip", "hk_rows_api.cpp"]
 
 
 def _compile(src: str) -> str:

@@ -623,16 +623,6 @@ extern "C" int hk_gemv_lowrank(hk_ctx* ctx, const hk_organ* left, const hk_organ
     return rc ? rc : hk_gemv(ctx, left, mid, y, stream);
 }
 
-struct hk_organ_set {
-    OrganView* dev = nullptr;
-    ResView* res_dev = nullptr;  // HGRAVR02 sets: the residual table
-    uint32_t res_pieces = 0;     // the most record pieces of any organ's apply part
-    uint32_t res_pieces_256 = 0;  // the same for 256-row parts
-    uint32_t res8_pieces = 0, res8_pieces_256 = 0;  // the byte steps' (the fused GEMV's)
-    uint32_t n = 0;
-    OrganView first{};
-};
-
 extern "C" int hk_organ_set_create(hk_ctx* ctx, const hk_organ* const* organs, uint32_t n, hk_organ_set** out) {
     if (!ctx || !out) return HK_E_INVALID_ARG;
     *out = nullptr;

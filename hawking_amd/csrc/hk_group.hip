@@ -1,0 +1,334 @@
+// hk_group.hip -- rows grouped by an id (the experts of routed tokens, the
+// adapters of requests) and the weighted sum of a token's grouped rows.
+//
+// Grouping is a stable counting sort of n ids over n_groups + 1 keys (an id
+// outside [0, n_groups) has key n_groups): offsets[g] = ids with a smaller
+// key, an id's place = offsets[key] + earlier ids of the same key.  Places
+// come from counts in a fixed order, never from the order atomics arrive in.
+// It reads 4 n bytes and writes 8 n + 4 (n_groups + 1): for every n that a
+// batch has the bound is latency (a launch, two dependent passes over ids).
+#include "hk_rows.h"
+
+namespace hk {
+
+__device__ __forceinline__ uint32_t group_key(int32_t id, uint32_t G) { return (uint32_t)id < G ? (uint32_t)id : G; }
+
+// ------------------------------------------------------------------ few ids: a workgroup a key, one launch
+
+// Workgroup g reads all ids: the number of smaller keys is offsets[g], and
+// the ids of key g get their places in order.  Each wave takes a quarter of
+// the ids, so the second pass needs no barrier: a wave's first place is the
+// quarters before it, a lane's the equal lanes below it.
+__global__ void __launch_bounds__(256) group_scan_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t G,
+                                                         int32_t* __restrict__ offsets, int32_t* __restrict__ order,
+                                                         int32_t* __restrict__ pos) {
+    __shared__ uint32_t less_s[4], equal_s[4];
+    const uint32_t g = blockIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t quarter = ((n + 255u) / 256u) * 64u, i0 = wave * quarter, i1 = min(i0 + quarter, n);
+    uint32_t less = 0, equal = 0;
+    for (uint32_t i = i0 + lane; i < i0 + quarter; i += 256u) {
+        // four loads in flight (an index past the quarter re-reads the last id)
+        int32_t v[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) v[j] = ldg(ids + min(i + 64u * j, n - 1u));
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t k = i + 64u * j < i1 ? group_key(v[j], G) : 0xFFFFFFFFu;
+            less += (uint32_t)__popcll(__ballot(k < g));
+            equal += (uint32_t)__popcll(__ballot(k == g));
+        }
+    }
+    if (lane == 0) {
+        less_s[wave] = less;
+        equal_s[wave] = equal;
+    }
+    __syncthreads();
+    uint32_t at = less_s[0] + less_s[1] + less_s[2] + less_s[3];
+    if (threadIdx.x == 0) offsets[g] = (int32_t)at;
+    for (uint32_t w = 0; w < wave; ++w) at += equal_s[w];
+    if (equal == 0) return;
+    for (uint32_t i = i0 + lane; i < i0 + quarter; i += 64u) {
+        const bool mine = i < i1 && group_key(ldg(ids + i), G) == g;
+        const uint64_t b = __ballot(mine);
+        if (mine) {
+            const uint32_t p = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
+            order[p] = (int32_t)i;
+            pos[i] = g < G ? (int32_t)p : -1;
+        }
+        at += (uint32_t)__popcll(b);
+    }
+}
+
+// ------------------------------------------------------------------ many ids: counts a part, then places
+
+constexpr uint32_t GROUP_WAVE_IDS = 256;  // ids of a wave
+
+// part[b][key]: the ids of workgroup b's part with that key.
+template <int NW>
+__global__ void __launch_bounds__(64 * NW) group_count_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t G,
+                                                              uint32_t* __restrict__ part) {
+    extern __shared__ uint32_t cnt[];  // [G + 1]
+    for (uint32_t k = threadIdx.x; k <= G; k += 64u * NW) cnt[k] = 0;
+    __syncthreads();
+    const uint32_t i0 = blockIdx.x * (NW * GROUP_WAVE_IDS);
+    int32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = ldg(ids + min(i0 + threadIdx.x + 64u * NW * (uint32_t)j, n - 1u));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (i0 + threadIdx.x + 64u * NW * (uint32_t)j < n) atomicAdd(&cnt[group_key(v[j], G)], 1u);
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k <= G; k += 64u * NW) part[(size_t)blockIdx.x * (G + 1u) + k] = cnt[k];
+}
+
+// Places.  The workgroup sums the counts of all parts (a key's offset is the
+// sum over smaller keys) and of the parts before its own; its waves count
+// their own 256 ids in LDS (16-bit counters, two a word), the counts of the
+// waves before give each wave its first place of a key, and the wave then
+// walks its ids 64 at a time: equal lanes find each other by one ballot a bit
+// of the key, and the lowest of them advances the counter.
+template <int NW>
+__global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t G,
+                                                              uint32_t bits, const uint32_t* __restrict__ part,
+                                                              uint32_t parts, int32_t* __restrict__ offsets,
+                                                              int32_t* __restrict__ order, int32_t* __restrict__ pos) {
+    constexpr uint32_t NT = 64u * NW;
+    extern __shared__ uint32_t sm[];
+    __shared__ uint32_t wsum[NW];
+    const uint32_t keys = G + 1u, words = (keys + 1u) / 2u;
+    uint32_t* base = sm;               // [keys] first place of the key in this part
+    uint32_t* wcnt = sm + keys;        // [NW][words] 16-bit counters
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, b = blockIdx.x;
+    uint32_t* mine = wcnt + wave * words;
+    for (uint32_t k = tid; k < NW * words; k += NT) wcnt[k] = 0;
+
+    const uint32_t i0 = b * (NW * GROUP_WAVE_IDS) + wave * GROUP_WAVE_IDS;
+    uint32_t key[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t i = i0 + 64u * (uint32_t)j + lane;
+        const int32_t v = ldg(ids + min(i, n - 1u));
+        key[j] = i < n ? group_key(v, G) : 0xFFFFFFFFu;
+    }
+    // this part's first place of every key: keys in runs of NT, a scan a run
+    uint32_t run = 0;
+    for (uint32_t k0 = 0; k0 < keys; k0 += NT) {
+        const uint32_t k = k0 + tid;
+        uint32_t total = 0, before = 0;
+        if (k < keys) {
+#pragma unroll 8
+            for (uint32_t p = 0; p < parts; ++p) {
+                const uint32_t c = part[(size_t)p * keys + k];
+                total += c;
+                before += p < b ? c : 0u;
+            }
+        }
+        const uint32_t inc = wave_incl_scan(total);
+        __syncthreads();
+        if (lane == 63u) wsum[wave] = inc;
+        __syncthreads();
+        uint32_t off = run, all = 0;
+        for (uint32_t w = 0; w < (uint32_t)NW; ++w) {
+            if (w < wave) off += wsum[w];
+            all += wsum[w];
+        }
+        off += inc - total;
+        if (k < keys) {
+            base[k] = off + before;
+            if (b == 0) offsets[k] = (int32_t)off;
+        }
+        run += all;
+    }
+    // (the counters were cleared before the barriers above)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (key[j] != 0xFFFFFFFFu) atomicAdd(&mine[key[j] >> 1], 1u << (16u * (key[j] & 1u)));
+    __syncthreads();
+    for (uint32_t w = tid; w < words; w += NT) {
+        uint32_t sum = 0;  // at most NW * 256 ids a part: no carry between the halves
+#pragma unroll
+        for (uint32_t v = 0; v < (uint32_t)NW; ++v) {
+            const uint32_t c = wcnt[v * words + w];
+            wcnt[v * words + w] = sum;
+            sum += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool in = key[j] != 0xFFFFFFFFu;
+        uint64_t same = __ballot(in);
+        for (uint32_t t = 0; t < bits; ++t) {
+            const bool one = (key[j] >> t) & 1u;
+            const uint64_t s = __ballot(one);
+            same &= one ? s : ~s;
+        }
+        const uint32_t rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0u));
+        if (in) {
+            const uint32_t h = 16u * (key[j] & 1u);
+            const uint32_t p = base[key[j]] + ((mine[key[j] >> 1] >> h) & 0xFFFFu) + rank;
+            const uint32_t i = i0 + 64u * (uint32_t)j + lane;
+            order[p] = (int32_t)i;
+            pos[i] = key[j] < G ? (int32_t)p : -1;
+        }
+        wave_lds_sync();  // every lane has read the counters
+        if (in && rank == 0) atomicAdd(&mine[key[j] >> 1], (uint32_t)__popcll(same) << (16u * (key[j] & 1u)));
+        wave_lds_sync();
+    }
+}
+
+// Up to GROUP_SCAN_READS id reads in all the one-launch form: measured against
+// the two-launch form at 512 and 327680 ids (see the launcher's callers' bench).
+constexpr uint64_t GROUP_SCAN_READS = 1ull << 22;
+
+static bool group_scans(uint32_t n, uint32_t G) { return (uint64_t)n * (G + 1u) <= GROUP_SCAN_READS; }
+static uint32_t group_part_ids(uint32_t G) { return (G <= 2048u ? 16u : 4u) * GROUP_WAVE_IDS; }
+
+size_t group_rows_ws_bytes(uint32_t n, uint32_t G) {
+    if (n == 0 || group_scans(n, G)) return 0;
+    return (size_t)((n + group_part_ids(G) - 1u) / group_part_ids(G)) * (G + 1u) * 4u;
+}
+
+template <int NW>
+static hipError_t group_parts(const int32_t* ids, uint32_t n, uint32_t G, int32_t* offsets, int32_t* order, int32_t* pos,
+                              uint32_t* part, hipStream_t s) {
+    const uint32_t keys = G + 1u, parts = (n + NW * GROUP_WAVE_IDS - 1u) / (NW * GROUP_WAVE_IDS);
+    uint32_t bits = 0;
+    while ((G >> bits) != 0) ++bits;
+    const size_t lds = ((size_t)keys + (size_t)NW * ((keys + 1u) / 2u)) * 4u;
+    hipLaunchKernelGGL(group_count_kernel<NW>, dim3(parts), dim3(64 * NW), keys * 4u, s, ids, n, G, part);
+    hipLaunchKernelGGL(group_place_kernel<NW>, dim3(parts), dim3(64 * NW), lds, s, ids, n, G, bits, part, parts, offsets,
+                       order, pos);
+    return hipGetLastError();
+}
+
+hipError_t launch_group_rows(const int32_t* ids, uint32_t n, uint32_t G, int32_t* offsets, int32_t* order, int32_t* pos,
+                             void* ws, hipStream_t s) {
+    if (group_scans(n, G)) {
+        hipLaunchKernelGGL(group_scan_kernel, dim3(G + 1u), dim3(256), 0, s, ids, n, G, offsets, order, pos);
+        return hipGetLastError();
+    }
+    uint32_t* part = static_cast<uint32_t*>(ws);
+    return G <= 2048u ? group_parts<16>(ids, n, G, offsets, order, pos, part, s)
+                      : group_parts<4>(ids, n, G, offsets, order, pos, part, s);
+}
+
+// ------------------------------------------------------------------ weighted sum of a token's rows
+
+template <int TYPE>
+__device__ __forceinline__ float elem(const void* x, size_t at) {
+    if constexpr (TYPE == HK_T_F32) return ldg(static_cast<const float*>(x) + at);
+    const uint16_t h = ldg(static_cast<const uint16_t*>(x) + at);
+    return TYPE == HK_T_BF16 ? __builtin_bit_cast(float, (uint32_t)h << 16) : f16_bits_to_f32(h);
+}
+
+// V consecutive elements (16 bytes where V > 1).
+template <int TYPE, int V>
+__device__ __forceinline__ void elems(const void* x, size_t at, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = elem<TYPE>(x, at);
+    } else if constexpr (TYPE == HK_T_F32) {
+        const float4 f = ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + at));
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+        const uint4 w = ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at));
+        const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = TYPE == HK_T_BF16 ? __builtin_bit_cast(float, d[i] << 16) : f16_bits_to_f32((uint16_t)d[i]);
+            v[2 * i + 1] = TYPE == HK_T_BF16 ? __builtin_bit_cast(float, d[i] & 0xFFFF0000u) : f16_bits_to_f32((uint16_t)(d[i] >> 16));
+        }
+    }
+}
+
+__device__ __forceinline__ void put_elem(void* y, int type, size_t at, float v) {
+    if (type == HK_T_F32) static_cast<float*>(y)[at] = v;
+    else static_cast<uint16_t*>(y)[at] = type == HK_T_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+}
+
+// y_t = base_t + sum over r ascending of w[t, r] x[pos[t, r]] in f32, one
+// rounding: V columns a thread, the x rows of CHUNK routes in flight at once.
+// A position outside [0, n) adds nothing.  Bound by reading x once.
+template <int TYPE, int V>
+__global__ void __launch_bounds__(256) combine_kernel(const void* x, size_t xs, uint32_t n, const int32_t* __restrict__ pos,
+                                                      const float* __restrict__ w, uint32_t K, uint32_t cols,
+                                                      const void* base, int base_type, size_t bs, void* y, int y_type,
+                                                      size_t ys, uint32_t blocks) {
+    constexpr int CHUNK = 5;
+    const uint32_t t = blockIdx.x / blocks, c = ((blockIdx.x % blocks) * 256u + threadIdx.x) * V;
+    if (c >= cols) return;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    for (uint32_t r0 = 0; r0 < K; r0 += CHUNK) {
+        float v[CHUNK][V], wt[CHUNK];
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) {
+            const uint32_t r = min(r0 + (uint32_t)j, K - 1u);
+            const uint32_t p = (uint32_t)pos[(size_t)t * K + r];
+            const bool on = r0 + (uint32_t)j < K && p < n;
+            wt[j] = w[(size_t)t * K + r];
+            if (on) {
+                elems<TYPE, V>(x, (size_t)p * xs + c, v[j]);
+            } else {
+                wt[j] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = __builtin_fmaf(wt[j], v[j][i], acc[i]);
+    }
+    if (base) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const size_t at = (size_t)t * bs + c + i;
+            acc[i] += base_type == HK_T_F32 ? elem<HK_T_F32>(base, at) : base_type == HK_T_BF16 ? elem<HK_T_BF16>(base, at) : elem<HK_T_F16>(base, at);
+        }
+    }
+    // y may be base itself: a thread reads its columns before it writes them
+    if (V > 1 && y_type == HK_T_F32 && ys % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+            *reinterpret_cast<float4*>(static_cast<float*>(y) + (size_t)t * ys + c + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    } else if (V == 8 && y_type != HK_T_F32 && ys % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
+        uint32_t d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            d[i] = y_type == HK_T_BF16 ? f32_to_bf16_bits(acc[(2 * i) % V]) | ((uint32_t)f32_to_bf16_bits(acc[(2 * i + 1) % V]) << 16)
+                                       : f32_to_f16_bits(acc[(2 * i) % V]) | ((uint32_t)f32_to_f16_bits(acc[(2 * i + 1) % V]) << 16);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + (size_t)t * ys + c) = make_uint4(d[0], d[1], d[2], d[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) put_elem(y, y_type, (size_t)t * ys + c + i, acc[i]);
+    }
+}
+
+template <int TYPE>
+static hipError_t combine_go(const void* x, size_t xs, uint32_t n, const int32_t* pos, const float* w, uint32_t tokens,
+                             uint32_t K, uint32_t cols, const void* base, int base_type, size_t bs, void* y, int y_type,
+                             size_t ys, hipStream_t s) {
+    constexpr int V = TYPE == HK_T_F32 ? 4 : 8;
+    const bool vec = cols % V == 0 && xs % V == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    const uint32_t blocks = (cols + 256u * (vec ? V : 1) - 1u) / (256u * (vec ? V : 1));
+    if ((uint64_t)blocks * tokens > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
+    if (vec)
+        hipLaunchKernelGGL((combine_kernel<TYPE, V>), dim3(blocks * tokens), dim3(256), 0, s, x, xs, n, pos, w, K, cols, base,
+                           base_type, bs, y, y_type, ys, blocks);
+    else
+        hipLaunchKernelGGL((combine_kernel<TYPE, 1>), dim3(blocks * tokens), dim3(256), 0, s, x, xs, n, pos, w, K, cols, base,
+                           base_type, bs, y, y_type, ys, blocks);
+    return hipGetLastError();
+}
+
+hipError_t launch_combine_rows(const void* x, int x_type, size_t xs, uint32_t n, const int32_t* pos, const float* w,
+                               uint32_t tokens, uint32_t K, uint32_t cols, const void* base, int base_type, size_t bs, void* y,
+                               int y_type, size_t ys, hipStream_t s) {
+    if (x_type == HK_T_F32) return combine_go<HK_T_F32>(x, xs, n, pos, w, tokens, K, cols, base, base_type, bs, y, y_type, ys, s);
+    if (x_type == HK_T_BF16) return combine_go<HK_T_BF16>(x, xs, n, pos, w, tokens, K, cols, base, base_type, bs, y, y_type, ys, s);
+    return combine_go<HK_T_F16>(x, xs, n, pos, w, tokens, K, cols, base, base_type, bs, y, y_type, ys, s);
+}
+
+}  // namespace hk

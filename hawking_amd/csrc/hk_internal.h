@@ -261,6 +261,33 @@ __device__ __forceinline__ float wave_max(float v) {
     return lane63_f32(v);
 }
 
+// Inclusive prefix sum over the 64 lanes on the DPP network.
+__device__ __forceinline__ uint32_t wave_incl_scan(uint32_t v) {
+    v += (uint32_t)dpp_i32<DPP_ROW_SHR1, 0xF>(0, (int)v);
+    v += (uint32_t)dpp_i32<DPP_ROW_SHR2, 0xF>(0, (int)v);
+    v += (uint32_t)dpp_i32<DPP_ROW_SHR4, 0xF>(0, (int)v);
+    v += (uint32_t)dpp_i32<DPP_ROW_SHR8, 0xF>(0, (int)v);
+    v += (uint32_t)dpp_i32<DPP_ROW_BCAST15, 0xA>(0, (int)v);
+    v += (uint32_t)dpp_i32<DPP_ROW_BCAST31, 0xC>(0, (int)v);
+    return v;
+}
+
+// Orders LDS writes before later LDS reads of other lanes of the same wave
+// (a wave's LDS instructions execute in order; this keeps the compiler from
+// reordering them).
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// f32 -> bf16 bits, round to nearest even; a NaN stays one.
+__device__ __forceinline__ uint16_t f32_to_bf16_bits(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((b >> 16) | 0x40u);
+    return (uint16_t)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
+}
+
 // ------------------------------------------------------------------ host error plumbing
 
 struct Status {
@@ -443,4 +470,15 @@ struct hk_organ {
     void* mem = nullptr;
     size_t alloc_bytes = 0;
     size_t packed_bytes = 0;
+};
+
+// Organs of one kind and shape with their descriptors in device memory (hk_organ_set_create).
+struct hk_organ_set {
+    hk::OrganView* dev = nullptr;
+    hk::ResView* res_dev = nullptr;  // HGRAVR02 sets: the residual table
+    uint32_t res_pieces = 0;     // the most record pieces of any organ's apply part
+    uint32_t res_pieces_256 = 0;  // the same for 256-row parts
+    uint32_t res8_pieces = 0, res8_pieces_256 = 0;  // the byte steps' (the fused GEMV's)
+    uint32_t n = 0;
+    hk::OrganView first{};
 };

@@ -1,0 +1,228 @@
+// hk_lora.hip -- low-rank adapters of many requests beside a shared packed
+// projection: y_t = W x_t + s_a B_a (A_a x_t), a the adapter of row t.
+//
+// A bank holds the adapters of one projection, laid out once: A in the column
+// order of the projection's row images (so one image of x serves W and A) and
+// B in the order of its row tiles, both as f16 scaled by a power of two a
+// matrix (bf16 and f16 values are exact down to 2^-28 of the largest).  A
+// call is three launches: the images, A x (this file), and W x with B mid
+// added to the same sums before they are stored (rows_lora in
+// hk_rows_kernel.h), so y is written once and W x is never read back.
+#include "hk_rows.h"
+
+namespace hk {
+
+// ------------------------------------------------------------------ bank
+
+__device__ __forceinline__ float lora_value(const void* p, int type, size_t at) {
+    const uint16_t h = ldg(static_cast<const uint16_t*>(p) + at);
+    return type == HK_T_BF16 ? __builtin_bit_cast(float, (uint32_t)h << 16) : f16_bits_to_f32(h);
+}
+
+// Block 0 finds A's exponent, block 1 B's; block 0 writes rank and scale.
+__global__ void __launch_bounds__(1024) lora_exps_kernel(const void* a, const void* b, int type, uint32_t rank, uint32_t rows,
+                                                         uint32_t cols, float scale, LoraSlot* slot, uint32_t* status) {
+    __shared__ float red[16];
+    const bool second = blockIdx.x == 1;
+    const size_t n = (size_t)rank * (second ? rows : cols);
+    float m = 0.0f;
+    for (size_t i = threadIdx.x; i < n; i += 1024u) {
+        const float v = fabsf(lora_value(second ? b : a, type, i));
+        m = v <= 3.4e38f ? fmaxf(m, v) : INFINITY;  // a NaN fails the comparison
+    }
+    m = wave_max(m);
+    if ((threadIdx.x & 63u) == 0u) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
+    if (!isfinite(scale)) m = INFINITY;
+    int e = 0;
+    const bool bad = !isfinite(m);
+    if (!bad && m > 0.0f) {
+        (void)frexpf(m, &e);
+        e = 14 - e;
+    }
+    if (bad) atomicOr(status, ROWS_ERR_NONFINITE);
+    if (second) {
+        slot->b_exp = bad ? ROWS_EXP_BAD : e;
+    } else {
+        slot->a_exp = bad ? ROWS_EXP_BAD : e;
+        slot->rank = rank;
+        slot->scale = scale;
+    }
+}
+
+// One 16-byte chunk a thread: first the chunks of A, then those of B.
+__global__ void __launch_bounds__(256) lora_pack_kernel(const void* a, const void* b, int type, uint32_t rank, uint32_t rows,
+                                                        uint32_t cols, int kind, uint32_t stages, uint32_t kk_max,
+                                                        const LoraSlot* slot, uint8_t* a_out, uint8_t* b_out) {
+    const size_t na = (size_t)2u * kk_max * stages * 256u, nb = (size_t)n_tiles_for(rows) * kk_max * 64u;
+    size_t i = (size_t)blockIdx.x * 256u + threadIdx.x;
+    if (i >= na + nb) return;
+    const bool second = i >= na;
+    if (second) i -= na;
+    const uint32_t lane = (uint32_t)(i & 63u), q = lane >> 4;
+    const int32_t e = second ? slot->b_exp : slot->a_exp;
+    hk_f16x8 h;
+    if (!second) {
+        const uint32_t u = (uint32_t)(i >> 6) & 3u, s = (uint32_t)((i >> 8) % stages);
+        const uint32_t r = 16u * (uint32_t)((i >> 8) / stages) + (lane & 15u);
+        const RowsCols c = rows_chunk_cols(kind, s * 16u + u * 4u + q);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t col = c.c0 + c.s0 * (uint32_t)(k >> 1) + ((k & 1) ? c.s1 : 0u);
+            h[k] = (r < rank && col < cols && e != ROWS_EXP_BAD) ? (_Float16)ldexpf(lora_value(a, type, (size_t)r * cols + col), e)
+                                                                : (_Float16)0.0f;
+        }
+        *reinterpret_cast<hk_f16x8*>(a_out + i * 16u) = h;
+    } else {
+        const uint32_t kk = (uint32_t)((i >> 6) % kk_max), row = 16u * (uint32_t)((i >> 6) / kk_max) + (lane & 15u);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t r = 32u * kk + 8u * q + (uint32_t)k;
+            h[k] = (r < rank && row < rows && e != ROWS_EXP_BAD) ? (_Float16)ldexpf(lora_value(b, type, (size_t)row * rank + r), e)
+                                                                : (_Float16)0.0f;
+        }
+        *reinterpret_cast<hk_f16x8*>(b_out + i * 16u) = h;
+    }
+}
+
+hipError_t launch_lora_pack(const void* a, const void* b, int type, uint32_t rank, uint32_t rows, uint32_t cols, int kind,
+                            float scale, uint32_t slot, uint32_t kk_max, LoraSlot* tab, uint8_t* a_bank, uint8_t* b_bank,
+                            uint32_t* status, hipStream_t s) {
+    const uint32_t stages = rows_stages(kind, cols);
+    const size_t a_slot = (size_t)2u * kk_max * stages * 4096u, b_slot = (size_t)n_tiles_for(rows) * kk_max * 1024u;
+    hipLaunchKernelGGL(lora_exps_kernel, dim3(2), dim3(1024), 0, s, a, b, type, rank, rows, cols, scale, tab + slot, status);
+    if (rank == 0) return hipGetLastError();
+    const size_t n = (a_slot + b_slot) / 16u;
+    hipLaunchKernelGGL(lora_pack_kernel, dim3((uint32_t)((n + 255u) / 256u)), dim3(256), 0, s, a, b, type, rank, rows, cols, kind,
+                       stages, kk_max, tab + slot, a_bank + a_slot * slot, b_bank + b_slot * slot);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ A x
+
+// A workgroup: 16 positions of one slot, all RT rank tiles, the stages of the
+// image split over NW waves (wave w takes stages w, w + NW, ...) and summed
+// in wave order.  The first wave then holds whole mid rows: a row is scaled
+// by the power of two that brings its maximum into [2^13, 2^14) and stored as
+// f16 (planes = 2: with the rounding error as a second f16).  mid_exps is the
+// exponent of y's part: B mid = sums * 2^-mid_exps, kept at most 80 above the
+// row's own exponent so that W x fits f32 in those units.
+template <int XP, int RT, int NW>
+__global__ void __launch_bounds__(64 * NW) lora_shrink_kernel(RowsArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [NW - 1][RT][64]
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = threadIdx.x >> 6, m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
+    if (blockIdx.x >= *a.ws.n_tiles) return;
+    const RowsTile tile = a.ws.tiles[blockIdx.x];
+    const uint32_t p = min(tile.first + m, tile.last - 1u);
+    const LoraSlot slot = a.lora.tab[tile.group];
+    const uint32_t rt_used = min((slot.rank + 15u) / 16u, (uint32_t)RT);
+    uint32_t r = p;
+    if (a.order) r = (uint32_t)a.order[p] / a.per_row;
+    const bool bad = r >= a.n_src;
+    if (bad) r = 0;
+    const uint8_t* x = a.ws.img + (size_t)r * a.stages * (256u * XP) + 16u * q;
+    const uint8_t* w = a.lora.a + (size_t)tile.group * (2u * a.lora.kk_max) * a.stages * 4096u + 16u * (uint32_t)lane;
+    hk_f32x4 acc[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[i] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s = wave; s < a.stages; s += NW) {
+        hk_f16x8 xv[4][XP];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int pl = 0; pl < XP; ++pl)
+                xv[u][pl] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(x + (size_t)s * (256u * XP) + 256u * pl + 64u * u)));
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if ((uint32_t)i < rt_used) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const hk_f16x8 wv = __builtin_bit_cast(
+                        hk_f16x8, ldg(reinterpret_cast<const uint4*>(w + ((size_t)i * a.stages + s) * 4096u + 1024u * u)));
+                    acc[i] = rows_mfma<1, XP>(wv, wv, xv[u], acc[i]);
+                }
+            }
+        }
+    }
+    if (wave) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) part[((wave - 1u) * RT + i) * 64u + lane] = acc[i];
+    }
+    __syncthreads();
+    if (wave) return;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        for (uint32_t k = 0; k + 1u < (uint32_t)NW; ++k) acc[i] += part[(k * RT + i) * 64u + lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[i][j] *= slot.scale;
+            top = fmaxf(top, fabsf(acc[i][j]));
+        }
+    }
+    // the row's four lanes
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (tile.first + m >= tile.last) return;
+    const int32_t E = a.ws.exps[r];
+    const bool nan = bad || E == ROWS_EXP_BAD || slot.a_exp == ROWS_EXP_BAD || slot.b_exp == ROWS_EXP_BAD || !isfinite(top);
+    int g = 0, out = 0;
+    if (!nan) {
+        out = E;
+        if (top > 0.0f) {
+            int e;
+            (void)frexpf(top, &e);
+            g = 14 - e;
+            out = g + E + slot.a_exp + slot.b_exp;
+            if (out > E + 80) {
+                g -= out - (E + 80);
+                out = E + 80;
+            }
+        }
+    }
+    if (q == 0) {
+        a.lora.mid_exps[p] = nan ? ROWS_EXP_BAD : out;
+        if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
+    }
+    uint8_t* o = a.lora.mid + (size_t)p * a.lora.planes * a.lora.kk_max * 64u;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        if (16u * (uint32_t)i >= 32u * a.lora.kk_max) break;
+        uint16_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float v = nan ? 0.0f : ldexpf(acc[i][j], g);
+            h[j] = f32_to_f16_bits(v);
+            l[j] = f32_to_f16_bits(v - f16_bits_to_f32(h[j]));
+        }
+        uint8_t* at = o + 32u * i + 8u * q;
+        *reinterpret_cast<uint2*>(at) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+        if (a.lora.planes == 2)
+            *reinterpret_cast<uint2*>(at + a.lora.kk_max * 64u) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
+    }
+}
+
+template <int XP, int RT, int NW>
+static hipError_t shrink_go(const RowsArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((lora_shrink_kernel<XP, RT, NW>), dim3(a.ws.max_tiles), dim3(64 * NW), (size_t)(NW - 1) * RT * 1024u, s, a);
+    return hipGetLastError();
+}
+
+template <int XP>
+static hipError_t shrink_rank(const RowsArgs& a, hipStream_t s) {
+    const uint32_t tiles = 2u * a.lora.kk_max;
+    if (tiles <= 2) return shrink_go<XP, 2, 8>(a, s);
+    if (tiles <= 4) return shrink_go<XP, 4, 8>(a, s);
+    if (tiles <= 8) return shrink_go<XP, 8, 4>(a, s);
+    return shrink_go<XP, 16, 4>(a, s);
+}
+
+hipError_t launch_lora_shrink(const RowsArgs& a, int xp, hipStream_t s) {
+    return xp == 2 ? shrink_rank<2>(a, s) : shrink_rank<1>(a, s);
+}
+
+}  // namespace hk

@@ -37,26 +37,6 @@ size_t moe_batch_img_bytes(uint32_t cols) { return x_lds_bytes<HK_Q4>(n_steps_fo
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
 
-// Orders LDS writes before later LDS reads of other lanes of the same wave
-// (a wave's LDS instructions execute in order; this keeps the compiler from
-// reordering them).
-__device__ __forceinline__ void wave_lds_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// Inclusive prefix sum over the 64 lanes on the DPP network.
-__device__ __forceinline__ uint32_t wave_incl_scan(uint32_t v) {
-    v += (uint32_t)dpp_i32<DPP_ROW_SHR1, 0xF>(0, (int)v);
-    v += (uint32_t)dpp_i32<DPP_ROW_SHR2, 0xF>(0, (int)v);
-    v += (uint32_t)dpp_i32<DPP_ROW_SHR4, 0xF>(0, (int)v);
-    v += (uint32_t)dpp_i32<DPP_ROW_SHR8, 0xF>(0, (int)v);
-    v += (uint32_t)dpp_i32<DPP_ROW_BCAST15, 0xA>(0, (int)v);
-    v += (uint32_t)dpp_i32<DPP_ROW_BCAST31, 0xC>(0, (int)v);
-    return v;
-}
-
 // Selection key of any non-NaN float v at index i: the unsigned order of the
 // keys is (value desc, index asc); 0 = taken.
 __device__ __forceinline__ uint64_t order_key(float v, uint32_t i) {

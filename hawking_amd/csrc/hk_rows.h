@@ -1,0 +1,289 @@
+// hk_rows.h -- products of many rows with packed organs on the f16 matrix
+// cores: what the image, product and adapter kernels share.
+//
+// The GEMV engine (hk_mfma.h) multiplies one vector and is bound by the
+// weight stream.  With many rows the same weights serve a whole tile of rows
+// and the matrix cores become the bound, so the operands are:
+//
+//   * x as a row image: every row scaled by a power of two so that its
+//     largest magnitude lies in [2^13, 2^14), as f16.  bf16 and f16 rows fit
+//     one plane exactly (down to 2^-28 of the row's maximum, below that with
+//     an absolute error of 2^-39 of it); f32 rows take a second plane with
+//     the first one's rounding error (22 bits) where y is f32 or f16.
+//   * W decoded in registers from the tiled bytes (hk_tile.h): code values
+//     are exact in f16 and code * scale is rounded once to f16 (2^-12) where
+//     y is bf16 (2^-9), or held exactly as the sum of two f16 (the rounded
+//     product and what the rounding lost) where y is f32 or f16: a scale has
+//     11 bits and a code at most 8.  Binary weights (+-scale) are exact in one.
+//   * sums in f32, scaled back by the row's power of two at the end.
+//
+// Columns.  v_mfma_f32_16x16x32_f16 multiplies 32 columns; lane (n = l % 16,
+// q = l / 16) supplies 8 of them for row n of its operand.  Both operands may
+// take any 8 columns as long as they are the same ones, so a lane takes the
+// columns its weight bytes hold (no lane exchange, one scale a lane) and the
+// image stores x in that order: chunk (stage s, product u, slot q) = 16 bytes
+// at s * 256 + u * 64 + q * 16 of a plane.  A stage is four products.
+#pragma once
+
+#include "hk_internal.h"
+#include "hk_mfma.h"
+#include "hk_tile.h"
+
+namespace hk {
+
+typedef _Float16 hk_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hk_f16x8 __attribute__((ext_vector_type(8)));
+
+// device status bits (hk_check_device_status)
+constexpr uint32_t ROWS_ERR_NONFINITE = 1u, ROWS_ERR_ROUTE = 2u;
+
+// Columns of a superstep (one weight fetch) and its stages.
+template <int KIND>
+struct RowsCfg {
+    static constexpr int STAGES = 1;
+    static constexpr uint32_t COLS = 128;
+};
+template <>
+struct RowsCfg<HK_BIN> {
+    static constexpr int STAGES = 4;
+    static constexpr uint32_t COLS = 512;
+};
+template <>
+struct RowsCfg<HK_MIXED> {
+    static constexpr int STAGES = 4;
+    static constexpr uint32_t COLS = 512;
+};
+
+__host__ __device__ inline uint32_t rows_stages(int kind, uint32_t cols) {
+    return (kind == HK_BIN || kind == HK_MIXED) ? (cols + 511u) / 512u * 4u : (cols + 127u) / 128u;
+}
+
+// The columns of image chunk ch (16 bytes; 16 chunks a stage): elements 2k
+// and 2k + 1 are columns c0 + s0 k and c0 + s0 k + s1.
+//   Q4, U3  a dword holds 8 columns; masking it pairs nibble k with nibble
+//           k + 4 in the two halves of a register
+//   Q8      bytes are taken in order
+//   BIN, MIXED  bit i of a dword pairs with bit i + 16
+struct RowsCols {
+    uint32_t c0, s0, s1;
+};
+__host__ __device__ inline RowsCols rows_chunk_cols(int kind, uint32_t ch) {
+    const uint32_t q = ch & 3u, u = (ch >> 2) & 3u;
+    if (kind == HK_BIN || kind == HK_MIXED)
+        return {512u * (ch >> 6) + 128u * q + 32u * ((ch >> 4) & 3u) + 4u * u, 1u, 16u};
+    if (kind == HK_Q8) return {128u * (ch >> 4) + 64u * (u >> 1) + 16u * q + 8u * (u & 1u), 2u, 1u};
+    return {128u * (ch >> 4) + 32u * q + 8u * u, 1u, 4u};
+}
+
+// ------------------------------------------------------------------ weights
+
+// One superstep of one row tile as fetched.
+template <int KIND>
+struct RowsW {
+    Frag<KIND, 1> f[KIND == HK_Q8 ? 2 : 1];
+};
+
+// hdr: the mixed kind's header of superstep t, loaded ahead (unused by the others).
+template <int KIND>
+__device__ __forceinline__ void rows_fetch(const OrganView& o, uint32_t T, uint32_t t, int lane, const uint4& hdr,
+                                           RowsW<KIND>& w) {
+    if constexpr (KIND == HK_Q8) {
+        // a superstep is two steps; past the last step x is zero
+        fetch_one<HK_Q8, 1>(o, T, 2u * t, lane, w.f[0], 0);
+        fetch_one<HK_Q8, 1>(o, T, min(2u * t + 1u, o.steps - 1u), lane, w.f[1], 0);
+    } else if constexpr (KIND == HK_MIXED) {
+        fetch_mixed<1>(o, hdr, lane, w.f[0], 0);
+    } else {
+        fetch_one<KIND, 1>(o, T, t, lane, w.f[0], 0);
+    }
+}
+
+__device__ __forceinline__ hk_f16x2 h2_bits(uint32_t v) { return __builtin_bit_cast(hk_f16x2, v); }
+__device__ __forceinline__ hk_f16x2 h2_all(float v) { return hk_f16x2{(_Float16)v, (_Float16)v}; }
+__device__ __forceinline__ uint32_t both_halves(uint16_t s) { return (uint32_t)s | ((uint32_t)s << 16); }
+
+// This lane's 8 weights of product u of stage a: hi = code * scale rounded to
+// f16, and (WP = 2) lo = code * scale - hi, exact.  An integer n < 1024 in the
+// low mantissa bits of f16 1024 (0x6400) is the f16 number 1024 + n, so a
+// masked field becomes a number with one OR and one exact subtraction.
+template <int KIND, int WP>
+__device__ __forceinline__ void rows_weights(const RowsW<KIND>& w, int a, int u, hk_f16x8& hi, hk_f16x8& lo) {
+    hk_f16x2 c[4];
+    uint32_t s2;
+    if constexpr (KIND == HK_BIN) {
+        // bit set: +scale.  Bit i goes to the sign of the low half, bit i + 16 to the high half's
+        const uint32_t neg = both_halves(w.f[0].s[0]) ^ 0x80008000u;
+        const uint32_t v = (&w.f[0].v[0].x)[a];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const hk_f16x2 x = h2_bits(((v << (15 - 4 * u - k)) & 0x80008000u) ^ neg);
+            hi[2 * k] = x[0];
+            hi[2 * k + 1] = x[1];
+        }
+        return;
+    } else if constexpr (KIND == HK_Q4) {
+        const uint32_t v = (&w.f[0].v[0].x)[u], v8 = v >> 8;
+        const hk_f16x2 m8 = h2_all(-1032.0f), m72 = h2_all(-72.0f), r16 = h2_all(0.0625f);
+        c[0] = h2_bits((v & 0x000F000Fu) | 0x64006400u) + m8;
+        c[1] = __builtin_elementwise_fma(h2_bits((v & 0x00F000F0u) | 0x64006400u), r16, m72);
+        c[2] = h2_bits((v8 & 0x000F000Fu) | 0x64006400u) + m8;
+        c[3] = __builtin_elementwise_fma(h2_bits((v8 & 0x00F000F0u) | 0x64006400u), r16, m72);
+        s2 = both_halves(w.f[0].s[0]);
+    } else if constexpr (KIND == HK_U3) {
+        const uint32_t lw = u < 2 ? w.f[0].lo[0].x : w.f[0].lo[0].y;
+        const uint32_t v = (u & 1) ? lw >> 16 : lw;
+        const uint32_t vv = (v & 0xFFu) | ((v & 0xFF00u) << 8);
+        const uint32_t hb = w.f[0].hi[0] >> (8 * u), hh = (hb & 0xFu) | ((hb & 0xF0u) << 12);
+        const hk_f16x2 m = h2_all(-1027.0f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            c[k] = h2_bits(((vv >> (2 * k)) & 0x00030003u) | (((hh >> k) & 0x00010001u) << 2) | 0x64006400u) + m;
+        s2 = both_halves(w.f[0].s[0]);
+    } else if constexpr (KIND == HK_Q8) {
+        const Frag<HK_Q8, 1>& f = w.f[u >> 1];
+        const hk_f16x2 m = h2_all(-1151.0f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t v = (&f.v[0].x)[2 * (u & 1) + (k >> 1)];
+            // bytes 2 (k % 2) and the next one, each under the byte 0x64
+            c[k] = h2_bits(__builtin_amdgcn_perm(0x64646464u, v, (k & 1) ? 0x04030402u : 0x04010400u)) + m;
+        }
+        s2 = both_halves(f.s[0]);
+    } else {
+        static_assert(KIND == HK_MIXED, "kind");
+        // binary items: bits 0..31 of dword a; Q2 items: 2-bit fields, even
+        // columns in dword a and odd ones in dword a + 4, bit 7 inverted.
+        // The field goes to bits 2..3 of each half of f16 256 (0x5C00, one
+        // unit = 0.25), so 256 + code, and code - 1.5 (2 b - 1) is exact.
+        const bool q2 = __builtin_amdgcn_inverse_ballot_w64(w.f[0].q2m[0]);
+        const uint32_t v0 = w.f[0].V[0][a], v1 = w.f[0].V[0][4 + a];
+        const uint32_t e = q2 ? v0 ^ 0x80808080u : v0, o = q2 ? v1 ^ 0x80808080u : v0 >> 1;
+        const uint32_t mask = q2 ? 0x000C000Cu : 0x00040004u;
+        const hk_f16x2 A = q2 ? h2_all(1.0f) : h2_all(2.0f), B = q2 ? h2_all(-257.5f) : h2_all(-513.0f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = 4 * u + k, r = ((i & ~1) + 30) & 31;
+            const uint32_t x = (i & 1) ? o : e;
+            c[k] = __builtin_elementwise_fma(h2_bits((__builtin_amdgcn_alignbit(x, x, r) & mask) | 0x5C005C00u), A, B);
+        }
+        s2 = both_halves(a < 2 ? w.f[0].s0[0] : w.f[0].s1[0]);
+    }
+    const hk_f16x2 s = h2_bits(s2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const hk_f16x2 h = c[k] * s;
+        hi[2 * k] = h[0];
+        hi[2 * k + 1] = h[1];
+        if constexpr (WP == 2) {
+            const hk_f16x2 l = __builtin_elementwise_fma(c[k], s, -h);
+            lo[2 * k] = l[0];
+            lo[2 * k + 1] = l[1];
+        }
+    }
+}
+
+__device__ __forceinline__ hk_f32x4 mfma_f16(const hk_f16x8& a, const hk_f16x8& b, const hk_f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// acc += W x over one product: the f16 parts' products down to 2^-22 of the whole.
+template <int WP, int XP>
+__device__ __forceinline__ hk_f32x4 rows_mfma(const hk_f16x8& wh, const hk_f16x8& wl, const hk_f16x8* x, hk_f32x4 acc) {
+    acc = mfma_f16(wh, x[0], acc);
+    if constexpr (WP == 2) acc = mfma_f16(wl, x[0], acc);
+    if constexpr (XP == 2) acc = mfma_f16(wh, x[1], acc);
+    return acc;
+}
+
+// ------------------------------------------------------------------ arguments
+
+// A row's exponent that stands for a row with a non-finite value (its products are NaN).
+constexpr int32_t ROWS_EXP_BAD = INT32_MIN;
+
+struct RowsTile {
+    uint32_t group, first, last;  // positions [first, last)
+    uint32_t pad;
+};
+
+// The products' workspace, as carved by the host.
+struct RowsWs {
+    uint8_t* img;      // [source rows][stages][planes][256 bytes]
+    int32_t* exps;     // [source rows]
+    RowsTile* tiles;   // [max_tiles]
+    uint32_t* n_tiles;
+    uint32_t max_tiles;
+};
+
+// An adapter of a bank (hk_lora.hip): A and B are stored as f16 times 2^a_exp
+// and 2^b_exp (ROWS_EXP_BAD: a value was not finite).  rank 0: an empty slot.
+struct LoraSlot {
+    uint32_t rank;
+    int32_t a_exp, b_exp;
+    float scale;
+};
+constexpr uint32_t LORA_MAX_RANK = 256;
+
+// Adapters of a launch (hk_gemm_lora): slot s owns positions [offsets[s], offsets[s + 1]).
+struct RowsLora {
+    const int32_t* offsets;
+    const LoraSlot* tab;      // [slots]
+    const uint8_t* a;         // [slot][2 kk_max rank tiles][stage][product][lane] 16 bytes
+    const uint8_t* b;         // [slot][row tile][kk_max][lane] 16 bytes
+    uint8_t* mid;             // [position][planes][kk_max] 64 bytes
+    int32_t* mid_exps;        // [position]
+    uint32_t slots, kk_max, planes;
+};
+
+struct RowsArgs {
+    const OrganView* organs;  // [groups]
+    const OrganView* up;      // [groups], SwiGLU only
+    RowsWs ws;
+    const int32_t* order;     // position -> flat index, or null
+    uint32_t per_row;         // flat indexes of a source row
+    uint32_t n, n_src;        // positions, source rows
+    uint32_t groups, rows, n_row_tiles, stages;
+    void* y;
+    size_t y_stride;          // elements
+    int32_t y_type;
+    uint32_t y_vec;           // four rows may be stored at once
+    uint32_t scatter;         // y row = order[position] (else the position)
+    uint32_t row_blocks;
+    uint32_t* status;
+    RowsLora lora;
+};
+
+// How a product launch is shaped.
+struct RowsShape {
+    int kind;
+    int wp, xp;       // weight and x planes
+    int form;         // ROWS_PLAIN, ROWS_GLU, ROWS_LORA
+    int mt;           // 16-row tiles of positions
+    bool tile;        // the tile kernel (x in LDS), else the split kernel
+    uint32_t kw;      // split kernel: waves that share a row tile's columns
+};
+constexpr int ROWS_PLAIN = 0, ROWS_GLU = 1, ROWS_LORA = 2;
+
+hipError_t launch_rows_image(const void* x, int x_type, size_t x_stride, uint32_t n, uint32_t cols, int kind, int planes,
+                             const RowsWs& ws, const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                             uint32_t* status, hipStream_t s);
+// The adapters' first half, A_s x of every position with an adapter, into lora.mid.
+hipError_t launch_lora_shrink(const RowsArgs& a, int xp, hipStream_t s);
+// An adapter into slot `slot`; a [rank x cols], b [rows x rank] of `type` (device).
+hipError_t launch_lora_pack(const void* a, const void* b, int type, uint32_t rank, uint32_t rows, uint32_t cols, int kind,
+                            float scale, uint32_t slot, uint32_t kk_max, LoraSlot* tab, uint8_t* a_bank, uint8_t* b_bank,
+                            uint32_t* status, hipStream_t s);
+size_t group_rows_ws_bytes(uint32_t n, uint32_t groups);
+hipError_t launch_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order, int32_t* pos,
+                             void* ws, hipStream_t s);
+hipError_t launch_combine_rows(const void* x, int x_type, size_t xs, uint32_t n, const int32_t* pos, const float* w,
+                               uint32_t tokens, uint32_t per_row, uint32_t cols, const void* base, int base_type, size_t bs,
+                               void* y, int y_type, size_t ys, hipStream_t s);
+hipError_t launch_rows_product(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+// one translation unit a kind
+hipError_t launch_rows_q4(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+hipError_t launch_rows_q8(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+hipError_t launch_rows_u3(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+hipError_t launch_rows_bin(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+hipError_t launch_rows_mixed(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+
+}  // namespace hk

@@ -1,0 +1,299 @@
+// hk_rows_api.cpp -- C entry points of the row products (hk_rows.h): checks,
+// workspace layout and the choice of a launch's shape.
+#include <algorithm>
+
+#include "hk_rows.h"
+#include "hk_rows_args.h"
+
+using namespace hk;
+
+namespace {
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Launches go to the context's device whatever the caller's current one is.
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(const hk_ctx* ctx) {
+        int cur = -1;
+        if (hipGetDevice(&cur) == hipSuccess && cur != ctx->device && hipSetDevice(ctx->device) == hipSuccess) prev = cur;
+    }
+    ~OnDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+int fail(hk_ctx* ctx, const char* fn, const RowsCheck& c) { return set_error(ctx, c.code, std::string(fn) + ": " + c.msg); }
+
+bool exact_weights(int32_t y_type) { return y_type != HK_T_BF16; }
+int x_planes(int32_t x_type, int32_t y_type) { return x_type == HK_T_F32 && exact_weights(y_type) ? 2 : 1; }
+
+// The launch's shape by the rows a group has on average.
+//  split  up to 16 rows a tile, the columns over the waves: bound by the
+//         weights, many small workgroups
+//  tile   64 or 128 rows a tile through LDS: bound by the matrix cores
+RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t n, uint32_t groups, uint32_t rows,
+                    uint32_t stages) {
+    RowsShape sh{};
+    sh.kind = kind;
+    sh.form = form;
+    sh.wp = exact_weights(y_type) ? 2 : 1;
+    sh.xp = x_planes(x_type, y_type);
+    const uint32_t per = n / std::max(1u, std::min(groups, n));
+    if (per <= 16) {
+        sh.mt = 1;
+    } else if (per <= 64 || sh.xp == 2) {
+        sh.mt = 4;
+        sh.tile = true;
+    } else {
+        sh.mt = 8;
+        sh.tile = true;
+    }
+    // columns over as many waves as have a superstep each
+    const uint32_t supers = (kind == HK_BIN || kind == HK_MIXED) ? stages / 4u : stages;
+    sh.kw = supers >= 4 ? 4 : supers >= 2 ? 2 : 1;
+    (void)rows;
+    return sh;
+}
+
+uint32_t max_tiles(uint32_t n, uint32_t groups, uint32_t tile_rows) { return n / tile_rows + std::min(groups, n); }
+
+// Sections of a product's workspace: exps, tiles, images (and an adapter call's mid rows).
+struct WsLayout {
+    size_t exps = 0, tiles = 0, mid_exps = 0, mid = 0, img = 0, total = 0;
+};
+WsLayout ws_layout(uint32_t x_rows, uint32_t stages, int planes, uint32_t n, uint32_t groups, uint32_t kk_max, int mid_planes) {
+    WsLayout L;
+    size_t at = 256;  // the tile count
+    L.exps = at;
+    at += align256((size_t)x_rows * 4);
+    L.tiles = at;
+    at += align256((size_t)max_tiles(n, groups, 16) * sizeof(RowsTile));
+    if (kk_max) {
+        L.mid_exps = at;
+        at += align256((size_t)n * 4);
+        L.mid = at;
+        at += align256((size_t)n * kk_max * 64u * mid_planes);
+    }
+    L.img = at;
+    L.total = at + (size_t)x_rows * stages * 256u * planes;
+    return L;
+}
+
+RowsWs ws_views(void* ws, const WsLayout& L, uint32_t tiles) {
+    uint8_t* b = static_cast<uint8_t*>(ws);
+    return {b + L.img, reinterpret_cast<int32_t*>(b + L.exps), reinterpret_cast<RowsTile*>(b + L.tiles),
+            reinterpret_cast<uint32_t*>(b), tiles};
+}
+
+void set_y(RowsArgs* a, const hk_rows* y) {
+    a->y = y->data;
+    a->y_type = y->type;
+    a->y_stride = y->stride;
+    a->y_vec = y->stride % 4 == 0 && reinterpret_cast<uintptr_t>(y->data) % (4 * type_bytes(y->type)) == 0;
+}
+
+int grouped(hk_ctx* ctx, const char* fn, const hk_organ_set* set, const hk_organ_set* up, const hk_rows* x,
+            const int32_t* order, uint32_t per_row, const int32_t* offsets, const hk_rows* y, void* ws, size_t ws_bytes,
+            hk_stream stream) {
+    if (!ctx) return HK_E_INVALID_ARG;
+    if (!set) return set_error(ctx, HK_E_INVALID_ARG, std::string(fn) + ": NULL organ set");
+    const OrganView& f = set->first;
+    if (up && (up->n != set->n || up->first.kind != f.kind || up->first.rows != f.rows || up->first.cols != f.cols ||
+               up->first.group != f.group))
+        return set_error(ctx, HK_E_GEOMETRY, std::string(fn) + ": the gate and up sets must share kind, shape and size");
+    const int kind = set->res_dev || (up && up->res_dev) ? HK_BIN_RICE : f.kind;
+    const uint32_t stages = rows_stages(f.kind, f.cols);
+    const WsLayout L = x && y ? ws_layout(x->n, stages, x_planes(x->type, y->type), y->n, set->n, 0, 0) : WsLayout{};
+    const RowsCheck c = check_product(kind, f.rows, f.cols, x, order, per_row, offsets, y, ws, ws_bytes, L.total);
+    if (!c.ok()) return fail(ctx, fn, c);
+    if (y->n == 0) return HK_OK;
+    OnDevice on(ctx);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const RowsShape sh = shape_for(f.kind, up ? ROWS_GLU : ROWS_PLAIN, x->type, y->type, y->n, set->n, f.rows, stages);
+    RowsArgs a{};
+    a.organs = set->dev;
+    a.up = up ? up->dev : nullptr;
+    a.ws = ws_views(ws, L, max_tiles(y->n, set->n, 16u * sh.mt));
+    a.order = order;
+    a.per_row = order ? per_row : 1u;
+    a.n = y->n;
+    a.n_src = x->n;
+    a.groups = set->n;
+    a.rows = f.rows;
+    a.n_row_tiles = f.n_tiles;
+    a.stages = stages;
+    a.status = ctx->dev_status;
+    set_y(&a, y);
+    int rc = check_hip(ctx, launch_rows_image(x->data, x->type, x->stride, x->n, f.cols, f.kind, sh.xp, a.ws, offsets, set->n,
+                                              y->n, 16u * sh.mt, ctx->dev_status, st),
+                       "row image launch");
+    if (!rc) rc = check_hip(ctx, launch_rows_product(sh, a, st), "row product launch");
+    return rc;
+}
+
+}  // namespace
+
+struct hk_lora_bank {
+    int32_t kind = 0, group = 0;
+    uint32_t rows = 0, cols = 0, n_slots = 0, max_rank = 0, kk_max = 0;
+    LoraSlot* tab = nullptr;  // the allocation's start
+    uint8_t* a = nullptr;
+    uint8_t* b = nullptr;
+};
+
+extern "C" size_t hk_group_rows_workspace(uint32_t n, uint32_t n_groups) {
+    return n_groups == 0 || n_groups > 8192 ? 0 : group_rows_ws_bytes(n, n_groups);
+}
+
+extern "C" int hk_group_rows(hk_ctx* ctx, const int32_t* ids, uint32_t n, uint32_t n_groups, int32_t* offsets, int32_t* order,
+                             int32_t* pos, void* ws, size_t ws_bytes, hk_stream stream) {
+    if (!ctx) return HK_E_INVALID_ARG;
+    const RowsCheck c = check_group(ids, n, n_groups, offsets, order, pos, ws, ws_bytes, hk_group_rows_workspace(n, n_groups));
+    if (!c.ok()) return fail(ctx, "hk_group_rows", c);
+    OnDevice on(ctx);
+    return check_hip(ctx, launch_group_rows(ids, n, n_groups, offsets, order, pos, ws, static_cast<hipStream_t>(stream)),
+                     "row grouping launch");
+}
+
+extern "C" size_t hk_gemm_grouped_workspace(const hk_organ_set* set, uint32_t x_rows, int32_t x_type, uint32_t n,
+                                            int32_t y_type) {
+    if (!set) return 0;
+    return ws_layout(x_rows, rows_stages(set->first.kind, set->first.cols), x_planes(x_type, y_type), n, set->n, 0, 0).total;
+}
+
+extern "C" int hk_gemm_grouped(hk_ctx* ctx, const hk_organ_set* set, const hk_rows* x, const int32_t* order, uint32_t per_row,
+                               const int32_t* offsets, const hk_rows* y, void* ws, size_t ws_bytes, hk_stream stream) {
+    return grouped(ctx, "hk_gemm_grouped", set, nullptr, x, order, per_row, offsets, y, ws, ws_bytes, stream);
+}
+
+extern "C" int hk_gemm_grouped_swiglu(hk_ctx* ctx, const hk_organ_set* gate, const hk_organ_set* up, const hk_rows* x,
+                                      const int32_t* order, uint32_t per_row, const int32_t* offsets, const hk_rows* y, void* ws,
+                                      size_t ws_bytes, hk_stream stream) {
+    if (!ctx) return HK_E_INVALID_ARG;
+    if (!up) return set_error(ctx, HK_E_INVALID_ARG, "hk_gemm_grouped_swiglu: NULL organ set");
+    return grouped(ctx, "hk_gemm_grouped_swiglu", gate, up, x, order, per_row, offsets, y, ws, ws_bytes, stream);
+}
+
+extern "C" int hk_combine_rows(hk_ctx* ctx, const hk_rows* x, const int32_t* pos, const float* weights, uint32_t per_row,
+                               uint32_t cols, const hk_rows* base, const hk_rows* y, hk_stream stream) {
+    if (!ctx) return HK_E_INVALID_ARG;
+    const RowsCheck c = check_combine(x, pos, weights, per_row, cols, base, y);
+    if (!c.ok()) return fail(ctx, "hk_combine_rows", c);
+    if (y->n == 0) return HK_OK;
+    OnDevice on(ctx);
+    return check_hip(ctx, launch_combine_rows(x->data, x->type, x->stride, x->n, pos, weights, y->n, per_row, cols,
+                                              base ? base->data : nullptr, base ? base->type : 0, base ? base->stride : 0,
+                                              y->data, y->type, y->stride, static_cast<hipStream_t>(stream)),
+                     "row sum launch");
+}
+
+extern "C" int hk_lora_bank_create(hk_ctx* ctx, const hk_organ* organ, uint32_t n_slots, uint32_t max_rank, hk_lora_bank** out) {
+    if (!ctx || !out) return HK_E_INVALID_ARG;
+    *out = nullptr;
+    if (!organ) return set_error(ctx, HK_E_INVALID_ARG, "hk_lora_bank_create: NULL organ");
+    const RowsCheck c = check_bank(organ->res_dev ? HK_BIN_RICE : organ->view.kind, n_slots, max_rank);
+    if (!c.ok()) return fail(ctx, "hk_lora_bank_create", c);
+    OnDevice on(ctx);
+    hk_lora_bank* b = new hk_lora_bank();
+    b->kind = organ->view.kind;
+    b->group = organ->view.group;
+    b->rows = organ->view.rows;
+    b->cols = organ->view.cols;
+    b->n_slots = n_slots;
+    b->max_rank = max_rank;
+    b->kk_max = (max_rank + 31u) / 32u;
+    const size_t tab = align256(n_slots * sizeof(LoraSlot));
+    const size_t a = (size_t)n_slots * 2u * b->kk_max * rows_stages(b->kind, b->cols) * 4096u;
+    const size_t bb = (size_t)n_slots * organ->view.n_tiles * b->kk_max * 1024u;
+    void* m = nullptr;
+    if (hipMalloc(&m, tab + a + bb) != hipSuccess) {
+        delete b;
+        return set_error(ctx, HK_E_NOMEM, "hk_lora_bank_create: allocation failed");
+    }
+    b->tab = static_cast<LoraSlot*>(m);
+    b->a = static_cast<uint8_t*>(m) + tab;
+    b->b = b->a + a;
+    int rc = check_hip(ctx, hipMemset(m, 0, tab), "adapter table clear");
+    if (!rc) rc = check_hip(ctx, hipDeviceSynchronize(), "adapter table clear");
+    if (rc) {
+        (void)hipFree(m);
+        delete b;
+        return rc;
+    }
+    *out = b;
+    return HK_OK;
+}
+
+extern "C" int hk_lora_bank_free(hk_ctx* ctx, hk_lora_bank* bank) {
+    if (!ctx) return HK_E_INVALID_ARG;
+    if (!bank) return HK_OK;
+    const int rc = check_hip(ctx, hipFree(bank->tab), "hipFree (adapter bank)");
+    delete bank;
+    return rc;
+}
+
+extern "C" int hk_lora_bank_set(hk_ctx* ctx, hk_lora_bank* bank, uint32_t slot, uint32_t rank, const void* a, const void* b,
+                                int32_t type, float scale, hk_stream stream) {
+    if (!ctx) return HK_E_INVALID_ARG;
+    if (!bank) return set_error(ctx, HK_E_INVALID_ARG, "hk_lora_bank_set: NULL bank");
+    const RowsCheck c = check_adapter(bank->n_slots, bank->max_rank, slot, rank, a, b, type);
+    if (!c.ok()) return fail(ctx, "hk_lora_bank_set", c);
+    OnDevice on(ctx);
+    return check_hip(ctx, launch_lora_pack(a, b, type, rank, bank->rows, bank->cols, bank->kind, scale, slot, bank->kk_max,
+                                           bank->tab, bank->a, bank->b, ctx->dev_status, static_cast<hipStream_t>(stream)),
+                     "adapter pack launch");
+}
+
+extern "C" size_t hk_gemm_lora_workspace(const hk_lora_bank* bank, uint32_t n, int32_t x_type, int32_t y_type) {
+    if (!bank) return 0;
+    return ws_layout(n, rows_stages(bank->kind, bank->cols), x_planes(x_type, y_type), n, bank->n_slots, bank->kk_max,
+                     exact_weights(y_type) ? 2 : 1).total;
+}
+
+extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_bank* bank, const hk_rows* x,
+                            const int32_t* order, const int32_t* offsets, const hk_rows* y, void* ws, size_t ws_bytes,
+                            hk_stream stream) {
+    static const char* fn = "hk_gemm_lora";
+    if (!ctx) return HK_E_INVALID_ARG;
+    if (!organ || !bank) return set_error(ctx, HK_E_INVALID_ARG, "hk_gemm_lora: NULL organ or bank");
+    const OrganView& f = organ->view;
+    if (f.kind != bank->kind || f.group != bank->group || f.rows != bank->rows || f.cols != bank->cols)
+        return set_error(ctx, HK_E_GEOMETRY, "hk_gemm_lora: the bank was made for an organ of another kind or shape");
+    if (x && y && x->n != y->n) return set_error(ctx, HK_E_GEOMETRY, "hk_gemm_lora: x and y need as many rows");
+    const uint32_t stages = rows_stages(f.kind, f.cols);
+    const int mid_planes = y && exact_weights(y->type) ? 2 : 1;
+    const WsLayout L = x && y ? ws_layout(x->n, stages, x_planes(x->type, y->type), y->n, bank->n_slots, bank->kk_max, mid_planes)
+                              : WsLayout{};
+    const RowsCheck c = check_product(organ->res_dev ? HK_BIN_RICE : f.kind, f.rows, f.cols, x, order, 1, offsets, y, ws, ws_bytes,
+                                      L.total);
+    if (!c.ok()) return fail(ctx, fn, c);
+    if (y->n == 0) return HK_OK;
+    OnDevice on(ctx);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const RowsShape sh = shape_for(f.kind, ROWS_LORA, x->type, y->type, y->n, 1, f.rows, stages);
+    RowsArgs a{};
+    a.organs = static_cast<const OrganView*>(organ->view_dev);
+    // the adapters' first half works on tiles of 16 rows of one slot
+    a.ws = ws_views(ws, L, max_tiles(y->n, bank->n_slots, 16));
+    a.order = order;
+    a.per_row = 1;
+    a.n = y->n;
+    a.n_src = x->n;
+    a.groups = 1;
+    a.rows = f.rows;
+    a.n_row_tiles = f.n_tiles;
+    a.stages = stages;
+    a.scatter = 1;
+    a.status = ctx->dev_status;
+    set_y(&a, y);
+    uint8_t* b = static_cast<uint8_t*>(ws);
+    a.lora = {offsets, bank->tab, bank->a, bank->b, b + L.mid, reinterpret_cast<int32_t*>(b + L.mid_exps),
+              bank->n_slots, bank->kk_max, (uint32_t)mid_planes};
+    int rc = check_hip(ctx, launch_rows_image(x->data, x->type, x->stride, x->n, f.cols, f.kind, sh.xp, a.ws, offsets,
+                                              bank->n_slots, y->n, 16, ctx->dev_status, st),
+                       "row image launch");
+    if (!rc) rc = check_hip(ctx, launch_lora_shrink(a, sh.xp, st), "adapter launch");
+    if (!rc) rc = check_hip(ctx, launch_rows_product(sh, a, st), "row product launch");
+    return rc;
+}

@@ -1,0 +1,120 @@
+// hk_rows_args.h -- argument checks of the row products, as plain host code
+// without a device (the entry points call them before any launch, and they
+// can be run where there is no GPU).
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/hawking_hip.h"
+
+namespace hk {
+
+struct RowsCheck {
+    int code = HK_OK;
+    const char* msg = "";
+    bool ok() const { return code == HK_OK; }
+};
+inline RowsCheck rows_fail(int code, const char* msg) { return {code, msg}; }
+
+inline size_t type_bytes(int32_t t) { return t == HK_T_F32 ? 4 : 2; }
+inline bool type_known(int32_t t) { return t == HK_T_F32 || t == HK_T_BF16 || t == HK_T_F16; }
+
+// Bytes from a row array's first element to the end of its last.
+inline size_t rows_span(const hk_rows& r, uint32_t cols) {
+    return r.n ? ((size_t)(r.n - 1u) * r.stride + cols) * type_bytes(r.type) : 0;
+}
+inline bool spans_overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na && nb && x < y + nb && y < x + na;
+}
+
+inline RowsCheck check_rows(const hk_rows* r, uint32_t cols) {
+    if (!r) return rows_fail(HK_E_INVALID_ARG, "NULL rows");
+    if (!type_known(r->type)) return rows_fail(HK_E_UNSUPPORTED, "rows are HK_T_F32, HK_T_BF16 or HK_T_F16");
+    if (r->n > 0x7FFFFFFFu) return rows_fail(HK_E_UNSUPPORTED, "at most 2^31 - 1 rows");
+    if (r->n == 0) return {};
+    if (!r->data) return rows_fail(HK_E_INVALID_ARG, "NULL row data");
+    if (reinterpret_cast<uintptr_t>(r->data) % type_bytes(r->type))
+        return rows_fail(HK_E_INVALID_ARG, "row data is not aligned to its element type");
+    if (r->n > 1 && r->stride < cols) return rows_fail(HK_E_GEOMETRY, "row stride smaller than the row");
+    if (r->n > 1 && r->stride > ((size_t)1 << 60) / r->n) return rows_fail(HK_E_GEOMETRY, "row stride too large");
+    return {};
+}
+
+inline RowsCheck check_group(const int32_t* ids, uint32_t n, uint32_t groups, const int32_t* offsets, const int32_t* order,
+                             const int32_t* pos, const void* ws, size_t ws_bytes, size_t need) {
+    if (groups == 0 || groups > 8192) return rows_fail(HK_E_UNSUPPORTED, "n_groups must be in [1, 8192]");
+    if (n > 0x7FFFFFFFu) return rows_fail(HK_E_UNSUPPORTED, "at most 2^31 - 1 ids");
+    if (!offsets || (n && (!ids || !order || !pos))) return rows_fail(HK_E_INVALID_ARG, "NULL ids or outputs");
+    const size_t b = (size_t)n * 4u, ob = ((size_t)groups + 1u) * 4u;
+    if (spans_overlap(ids, b, offsets, ob) || spans_overlap(ids, b, order, b) || spans_overlap(ids, b, pos, b) ||
+        spans_overlap(order, b, pos, b) || spans_overlap(order, b, offsets, ob) || spans_overlap(pos, b, offsets, ob))
+        return rows_fail(HK_E_INVALID_ARG, "ids and outputs must not overlap");
+    if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 4))
+        return rows_fail(HK_E_INVALID_ARG, "workspace missing, misaligned or smaller than hk_group_rows_workspace");
+    return {};
+}
+
+// rows, cols: the organ's; n_groups: the set's organs.
+inline RowsCheck check_product(int kind, uint32_t rows, uint32_t cols, const hk_rows* x, const int32_t* order, uint32_t per_row,
+                               const int32_t* offsets, const hk_rows* y, const void* ws, size_t ws_bytes, size_t need) {
+    if (kind != HK_Q4 && kind != HK_Q8 && kind != HK_U3 && kind != HK_BIN && kind != HK_MIXED)
+        return rows_fail(HK_E_UNSUPPORTED, "organ kind has no row product (HK_F32 and HGRAVR02 have none)");
+    RowsCheck c = check_rows(x, cols);
+    if (c.ok()) c = check_rows(y, rows);
+    if (!c.ok()) return c;
+    if (!offsets) return rows_fail(HK_E_INVALID_ARG, "NULL offsets");
+    if (order && per_row == 0) return rows_fail(HK_E_INVALID_ARG, "per_row must be positive");
+    if (y->n == 0) return {};
+    if (x->n == 0) return rows_fail(HK_E_GEOMETRY, "no source rows for the positions");
+    if (!order && x->n < y->n) return rows_fail(HK_E_GEOMETRY, "without order x needs a row for every row of y");
+    if (spans_overlap(x->data, rows_span(*x, cols), y->data, rows_span(*y, rows)))
+        return rows_fail(HK_E_INVALID_ARG, "x and y must not overlap");
+    if (!ws || reinterpret_cast<uintptr_t>(ws) % 256 || ws_bytes < need)
+        return rows_fail(HK_E_INVALID_ARG, "workspace missing, not 256-byte aligned or too small");
+    if (spans_overlap(ws, need, x->data, rows_span(*x, cols)) || spans_overlap(ws, need, y->data, rows_span(*y, rows)))
+        return rows_fail(HK_E_INVALID_ARG, "the workspace must not overlap x or y");
+    return {};
+}
+
+inline RowsCheck check_combine(const hk_rows* x, const int32_t* pos, const float* w, uint32_t per_row, uint32_t cols,
+                               const hk_rows* base, const hk_rows* y) {
+    if (cols == 0 || per_row == 0) return rows_fail(HK_E_GEOMETRY, "cols and per_row must be positive");
+    RowsCheck c = check_rows(x, cols);
+    if (c.ok()) c = check_rows(y, cols);
+    if (c.ok() && base) c = check_rows(base, cols);
+    if (!c.ok()) return c;
+    if (y->n == 0) return {};
+    if (!pos || !w) return rows_fail(HK_E_INVALID_ARG, "NULL pos or weights");
+    if (base && base->n < y->n) return rows_fail(HK_E_GEOMETRY, "base has fewer rows than y");
+    if (spans_overlap(x->data, rows_span(*x, cols), y->data, rows_span(*y, cols)))
+        return rows_fail(HK_E_INVALID_ARG, "x and y must not overlap");
+    if (base && spans_overlap(base->data, rows_span(*base, cols), y->data, rows_span(*y, cols)) &&
+        !(base->data == y->data && base->type == y->type && (base->stride == y->stride || y->n == 1)))
+        return rows_fail(HK_E_INVALID_ARG, "base may be y itself, but not overlap it otherwise");
+    return {};
+}
+
+inline RowsCheck check_bank(int kind, uint32_t n_slots, uint32_t max_rank) {
+    if (kind != HK_Q4 && kind != HK_Q8 && kind != HK_U3 && kind != HK_BIN && kind != HK_MIXED)
+        return rows_fail(HK_E_UNSUPPORTED, "organ kind has no row product (HK_F32 and HGRAVR02 have none)");
+    if (n_slots == 0 || n_slots > 8192) return rows_fail(HK_E_UNSUPPORTED, "n_slots must be in [1, 8192]");
+    if (max_rank == 0 || max_rank > 256) return rows_fail(HK_E_UNSUPPORTED, "max_rank must be in [1, 256]");
+    return {};
+}
+
+inline RowsCheck check_adapter(uint32_t n_slots, uint32_t max_rank, uint32_t slot, uint32_t rank, const void* a, const void* b,
+                               int32_t type) {
+    if (slot >= n_slots) return rows_fail(HK_E_INVALID_ARG, "slot outside the bank");
+    if (rank > max_rank) return rows_fail(HK_E_GEOMETRY, "rank above the bank's max_rank");
+    if (rank == 0) return {};
+    if (type != HK_T_BF16 && type != HK_T_F16) return rows_fail(HK_E_UNSUPPORTED, "adapters are HK_T_BF16 or HK_T_F16");
+    if (!a || !b || reinterpret_cast<uintptr_t>(a) % 2 || reinterpret_cast<uintptr_t>(b) % 2)
+        return rows_fail(HK_E_INVALID_ARG, "adapter arrays missing or misaligned");
+    return {};
+}
+
+}  // namespace hk

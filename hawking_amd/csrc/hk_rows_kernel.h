@@ -1,0 +1,473 @@
+// hk_rows_kernel.h -- the product kernels of hk_rows.h; each kind is
+// instantiated in a translation unit of its own (hk_rows_<kind>.hip).
+//
+// Both kernels multiply a tile of 16 MT positions of one group with row tiles
+// of the group's organ.  The weights are the MFMA's A operand (its 16 rows)
+// and the image the B operand (16 positions), so a lane ends with four
+// consecutive rows of one position.
+#pragma once
+
+#include "hk_rows.h"
+
+namespace hk {
+
+// The work item of this workgroup: position tile and row block.  Workgroups
+// go to the 8 XCDs round robin; each XCD takes one contiguous run of items
+// (row blocks of a position tile, then the next tile), so the row blocks that
+// read the same x rows share its L2.
+__device__ __forceinline__ bool rows_item(const RowsArgs& a, uint32_t n_tiles, uint32_t* tile, uint32_t* block) {
+    const uint32_t items = n_tiles * a.row_blocks, per = (items + 7u) / 8u;
+    const uint32_t k = blockIdx.x >> 3, i = (blockIdx.x & 7u) * per + k;
+    *tile = i / a.row_blocks;
+    *block = i % a.row_blocks;
+    return k < per && i < items;
+}
+
+// Position p's source row in the image; an index outside the source marks the
+// row bad (its results become NaN, as a non-finite row's).
+__device__ __forceinline__ uint32_t rows_source(const RowsArgs& a, uint32_t p, bool* bad) {
+    uint32_t r = p;
+    if (a.order) r = (uint32_t)a.order[p] / a.per_row;
+    *bad = r >= a.n_src;
+    return *bad ? 0u : r;
+}
+
+// Rows row .. row + 3 of y's row `yr`.
+__device__ __forceinline__ void rows_store(const RowsArgs& a, uint32_t yr, uint32_t row, const float (&v)[4]) {
+    const size_t at = (size_t)yr * a.y_stride + row;
+    if (a.y_vec && row + 4u <= a.rows) {
+        if (a.y_type == HK_T_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = a.y_type == HK_T_BF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (row + (uint32_t)i >= a.rows) return;
+        if (a.y_type == HK_T_F32) static_cast<float*>(a.y)[at + i] = v[i];
+        else static_cast<uint16_t*>(a.y)[at + i] = a.y_type == HK_T_BF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
+    }
+}
+
+// The adapters' part: acc (units of 2^-exps) is moved to the units of the
+// position's mid row and B_s mid is added for every slot s with positions in
+// the tile [first, last); the other positions' mid counts as zero.  T: the
+// RT row tiles of this wave; exps: this lane's position of every 16, updated.
+template <int MT, int RT>
+__device__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane, int32_t* exps,
+                          hk_f32x4 (&acc)[MT][RT]) {
+    const RowsLora& L = a.lora;
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
+    const size_t pitch = (size_t)L.kk_max * 64u * L.planes;
+    for (uint32_t s0 = 0; s0 < L.slots; s0 += 64u) {
+        const uint32_t sl = s0 + (uint32_t)lane;
+        uint32_t o0 = 0, o1 = 0;
+        if (sl < L.slots) {
+            o0 = min((uint32_t)max(L.offsets[sl], 0), a.n);
+            o1 = min((uint32_t)max(L.offsets[sl + 1], 0), a.n);
+        }
+        uint64_t hit = __ballot(o0 < last && o1 > first && o0 < o1);
+        while (hit) {
+            const int i = __builtin_ctzll(hit);
+            hit &= hit - 1;
+            const uint32_t s = s0 + (uint32_t)i;
+            const uint32_t lo = max(__builtin_amdgcn_readlane(o0, i), first), hi = min(__builtin_amdgcn_readlane(o1, i), last);
+            const uint32_t kk = min((L.tab[s].rank + 31u) / 32u, L.kk_max);
+            if (!kk) continue;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const uint32_t p = first + 16u * mt + m;
+                if (p >= lo && p < hi) {
+                    const int32_t g = L.mid_exps[p];
+                    const bool nan = exps[mt] == ROWS_EXP_BAD || g == ROWS_EXP_BAD;
+                    const int d = nan ? 0 : g - exps[mt];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[mt][r][j] = ldexpf(acc[mt][r][j], d);
+                    exps[mt] = nan ? ROWS_EXP_BAD : g;
+                }
+            }
+            for (uint32_t k = 0; k < kk; ++k) {
+                hk_f16x8 w[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    w[r] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
+                                                            L.b + (((size_t)s * a.n_row_tiles + T[r]) * L.kk_max + k) * 1024u + 16u * (uint32_t)lane)));
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint32_t t0 = first + 16u * mt;
+                    if (t0 >= hi || t0 + 16u <= lo) continue;  // uniform
+                    const uint32_t p = t0 + m;
+                    const bool mine = p >= lo && p < hi;
+                    for (uint32_t pl = 0; pl < L.planes; ++pl) {
+                        uint4 v = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)(mine ? p : lo) * pitch +
+                                                                     ((size_t)pl * L.kk_max + k) * 64u + 16u * q));
+                        if (!mine) v = make_uint4(0u, 0u, 0u, 0u);
+                        const hk_f16x8 x = __builtin_bit_cast(hk_f16x8, v);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(w[r], x, acc[mt][r]);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Scales a tile's sums back and stores them; GLU: row tiles r and r + RT / 2
+// are the gate and the up rows of the same outputs.
+template <int MT, int RT, bool GLU>
+__device__ __forceinline__ void rows_epilogue(const RowsArgs& a, uint32_t first, uint32_t last, uint32_t T0, int lane,
+                                              const int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
+    constexpr int RO = GLU ? RT / 2 : RT;
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
+    bool bad = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const uint32_t p = first + 16u * mt + m;
+        if (p >= last) continue;
+        uint32_t yr = p;
+        if (a.scatter && a.order) yr = (uint32_t)a.order[p];
+        if (yr >= a.n) continue;  // flagged by the staging
+        const bool nan = exps[mt] == ROWS_EXP_BAD;
+#pragma unroll
+        for (int r = 0; r < RO; ++r) {
+            const uint32_t row = 16u * (T0 + (uint32_t)r) + 4u * q;
+            if (row >= a.rows) continue;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x = nan ? __builtin_nanf("") : ldexpf(acc[mt][r][j], -exps[mt]);
+                if constexpr (GLU) {
+                    const float up = ldexpf(acc[mt][r + RO][j], -exps[mt]);
+                    x = x / (1.0f + expf(-x)) * up;
+                }
+                bad |= !isfinite(x);
+                v[j] = x;
+            }
+            rows_store(a, yr, row, v);
+        }
+    }
+    if (__ballot(bad) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
+}
+
+// ------------------------------------------------------------------ many rows a group: x through LDS
+
+// A workgroup of four waves: 16 MT positions x 16 row tiles (four a wave;
+// SwiGLU: two gate and two up).  Per stage (128 columns) the positions' image
+// is copied into one of two LDS buffers while the other is multiplied, with
+// one barrier a stage; each wave decodes its own weights in registers, so a
+// fragment of 16 rows x 32 columns serves MT products.  The 16-byte chunks of
+// a row are stored at chunk ^ (row % 16), so the 16 rows that a fragment read
+// touches lie in 16 different bank groups.
+template <int KIND, int WP, int XP, int MT, int FORM>
+__global__ void __launch_bounds__(256, 2) rows_tile_kernel(RowsArgs a) {
+    constexpr int RT = 4, BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
+    constexpr bool GLU = FORM == ROWS_GLU;
+    constexpr uint32_t BUF = BM * 256u * XP;
+    extern __shared__ __align__(16) uint8_t lds[];  // 2 BUF
+    __shared__ uint32_t src[BM];
+    __shared__ int32_t sexp[BM];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = threadIdx.x >> 6, tid = threadIdx.x;
+
+    uint32_t tile, block, group = 0, first, last;
+    if constexpr (FORM == ROWS_LORA) {
+        if (!rows_item(a, (a.n + BM - 1u) / BM, &tile, &block)) return;
+        first = tile * BM;
+        last = min(first + BM, a.n);
+    } else {
+        if (!rows_item(a, *a.ws.n_tiles, &tile, &block)) return;
+        const RowsTile t = a.ws.tiles[tile];
+        group = __builtin_amdgcn_readfirstlane(t.group);
+        first = __builtin_amdgcn_readfirstlane(t.first);
+        last = __builtin_amdgcn_readfirstlane(t.last);
+    }
+    if (tid < (uint32_t)BM) {
+        bool bad = false;
+        const uint32_t p = min(first + tid, last - 1u), r = rows_source(a, p, &bad);
+        src[tid] = r;
+        sexp[tid] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
+        if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
+    }
+    __syncthreads();
+
+    const OrganView o = a.organs[group];
+    const OrganView ou = GLU ? a.up[group] : o;
+    const uint32_t T0 = (block * 4u + wave) * (GLU ? RT / 2 : RT);
+    uint32_t T[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) T[r] = min(T0 + (uint32_t)(GLU ? r % (RT / 2) : r), a.n_row_tiles - 1u);
+    auto view = [&](int r) -> const OrganView& { return (GLU && r >= RT / 2) ? ou : o; };
+
+    // x: this thread copies chunk tid % 16 of rows tid / 16 + 16 i
+    const size_t pitch = (size_t)a.stages * 256u * XP;
+    const uint8_t* xs[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xs[i] = a.ws.img + (size_t)src[(tid >> 4) + 16u * i] * pitch + (tid & 15u) * 16u;
+    const uint32_t xd = (tid >> 4) * 256u + (((tid & 15u) ^ (tid >> 4)) * 16u);
+    uint4 xr[MT][XP];
+    auto x_load = [&](uint32_t s) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int p = 0; p < XP; ++p) xr[i][p] = ldg(reinterpret_cast<const uint4*>(xs[i] + (size_t)s * (256u * XP) + 256u * p));
+    };
+    auto x_store = [&](uint32_t s) {
+        uint8_t* b = lds + (s & 1u) * BUF + xd;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int p = 0; p < XP; ++p) *reinterpret_cast<uint4*>(b + p * (BM * 256u) + i * 4096u) = xr[i][p];
+    };
+
+    const uint32_t n_super = a.stages / STG;
+    uint4 hdr[RT] = {};
+    auto heads = [&](uint32_t t) {
+        if constexpr (KIND == HK_MIXED) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) hdr[r] = ldg(view(r).hdr + (T[r] * view(r).steps + t));
+        }
+    };
+    RowsW<KIND> cur[RT], nxt[RT];
+    auto w_load = [&](uint32_t t, RowsW<KIND>(&w)[RT]) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) rows_fetch<KIND>(view(r), T[r], t, lane, hdr[r], w[r]);
+    };
+
+    hk_f32x4 acc[MT][RT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    x_load(0);
+    heads(0);
+    w_load(0, cur);
+    heads(min(1u, n_super - 1u));
+    x_store(0);
+    __syncthreads();
+
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
+    for (uint32_t t = 0; t < n_super; ++t) {
+        w_load(min(t + 1u, n_super - 1u), nxt);
+        heads(min(t + 2u, n_super - 1u));
+#pragma unroll
+        for (int st = 0; st < STG; ++st) {
+            const uint32_t s = t * STG + st;
+            x_load(min(s + 1u, a.stages - 1u));
+            const uint8_t* b = lds + (s & 1u) * BUF + m * 256u;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint8_t* bu = b + (((4u * u + q) ^ m) * 16u);
+                hk_f16x8 x[MT][XP];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int p = 0; p < XP; ++p)
+                        x[mt][p] = *reinterpret_cast<const hk_f16x8*>(bu + p * (BM * 256u) + mt * 4096u);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    hk_f16x8 wh, wl;
+                    rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[mt], acc[mt][r]);
+                }
+            }
+            // the other buffer was last read before the previous stage's barrier
+            x_store(s + 1u);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
+    }
+
+    int32_t exps[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) exps[mt] = sexp[16 * mt + m];
+    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
+    rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
+}
+
+// ------------------------------------------------------------------ few rows a group: columns split over the waves
+
+// A workgroup of four waves: 16 MT positions x (4 / kw) pairs of row tiles;
+// kw waves share a pair, wave w of them taking supersteps w, w + kw, ... and
+// their sums are added in LDS in wave order.  Such calls are bound by the
+// weight stream and its latency: the image is read straight from L2 (each
+// wave's reads equal its weights' decoded size), without LDS or barriers in
+// the loop, and many small workgroups keep the loads in flight.
+template <int KIND, int WP, int XP, int MT, int FORM>
+__global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsArgs a, uint32_t kw) {
+    constexpr int RT = 2, BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
+    constexpr bool GLU = FORM == ROWS_GLU;
+    __shared__ hk_f32x4 part[3][MT * RT][64];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = threadIdx.x >> 6, wk = wave % kw, wr = wave / kw;
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
+
+    uint32_t tile, block, group = 0, first, last;
+    if constexpr (FORM == ROWS_LORA) {
+        if (!rows_item(a, (a.n + BM - 1u) / BM, &tile, &block)) return;
+        first = tile * BM;
+        last = min(first + BM, a.n);
+    } else {
+        if (!rows_item(a, *a.ws.n_tiles, &tile, &block)) return;
+        const RowsTile t = a.ws.tiles[tile];
+        group = __builtin_amdgcn_readfirstlane(t.group);
+        first = __builtin_amdgcn_readfirstlane(t.first);
+        last = __builtin_amdgcn_readfirstlane(t.last);
+    }
+    const OrganView o = a.organs[group];
+    const OrganView ou = GLU ? a.up[group] : o;
+    const uint32_t T0 = (block * (4u / kw) + wr) * (GLU ? RT / 2 : RT);
+    uint32_t T[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) T[r] = min(T0 + (uint32_t)(GLU ? r % (RT / 2) : r), a.n_row_tiles - 1u);
+    auto view = [&](int r) -> const OrganView& { return (GLU && r >= RT / 2) ? ou : o; };
+
+    const size_t pitch = (size_t)a.stages * 256u * XP;
+    const uint8_t* xs[MT];
+    int32_t exps[MT];
+    bool any_bad = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        bool bad = false;
+        const uint32_t r = rows_source(a, min(first + 16u * mt + m, last - 1u), &bad);
+        xs[mt] = a.ws.img + (size_t)r * pitch + 16u * q;
+        exps[mt] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
+        any_bad |= bad;
+    }
+    if (__ballot(any_bad) && lane == 0) atomicOr(a.status, ROWS_ERR_ROUTE);
+
+    hk_f32x4 acc[MT][RT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const uint32_t n_super = a.stages / STG;
+    uint4 hdr[RT] = {};
+    auto heads = [&](uint32_t t) {
+        if constexpr (KIND == HK_MIXED) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) hdr[r] = ldg(view(r).hdr + (T[r] * view(r).steps + min(t, n_super - 1u)));
+        }
+    };
+    RowsW<KIND> cur[RT], nxt[RT];
+    auto w_load = [&](uint32_t t, RowsW<KIND>(&w)[RT]) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) rows_fetch<KIND>(view(r), T[r], min(t, n_super - 1u), lane, hdr[r], w[r]);
+    };
+    if (wk < n_super) {
+        heads(wk);
+        w_load(wk, cur);
+        heads(wk + kw);
+        for (uint32_t t = wk; t < n_super; t += kw) {
+            w_load(t + kw, nxt);
+            heads(t + 2u * kw);
+#pragma unroll
+            for (int st = 0; st < STG; ++st) {
+                const size_t off = (size_t)(t * STG + st) * (256u * XP);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    hk_f16x8 x[MT][XP];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int p = 0; p < XP; ++p)
+                            x[mt][p] = __builtin_bit_cast(
+                                hk_f16x8, ldg(reinterpret_cast<const uint4*>(xs[mt] + off + 256u * p + 64u * u)));
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        hk_f16x8 wh, wl;
+                        rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[mt], acc[mt][r]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
+        }
+    }
+    if (kw > 1) {
+        // part[wave - wr - 1]: the waves that are not their pair's first
+        if (wk) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) part[wave - wr - 1u][mt * RT + r][lane] = acc[mt][r];
+        }
+        __syncthreads();
+        if (wk) return;
+        for (uint32_t k = 1; k < kw; ++k)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[mt][r] += part[wave + k - wr - 1u][mt * RT + r][lane];
+    }
+    if (T0 >= a.n_row_tiles) return;
+    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
+    rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
+}
+
+// ------------------------------------------------------------------ launch
+
+template <int KIND, int WP, int XP, int MT, int FORM>
+hipError_t rows_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
+    constexpr uint32_t out_tiles = FORM == ROWS_GLU ? 2u : 1u;  // tiles per output tile
+    const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles;
+    const uint32_t per = sh.tile ? 16u / out_tiles : 4u / sh.kw * 2u / out_tiles;
+    a.row_blocks = (a.n_row_tiles + per - 1u) / per;
+    const uint64_t items = (uint64_t)tiles * a.row_blocks, grid = (items + 7u) / 8u * 8u;
+    if (grid == 0) return hipSuccess;
+    if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
+    if (sh.tile) {
+        constexpr size_t lds = 2u * 16u * MT * 256u * XP;
+        auto* k = rows_tile_kernel<KIND, WP, XP, MT, FORM>;
+        hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), lds, s, a);
+    } else {
+        auto* k = rows_split_kernel<KIND, WP, XP, MT, FORM>;
+        hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), 0, s, a, sh.kw);
+    }
+    return hipGetLastError();
+}
+
+template <int KIND, int WP, int XP, int FORM>
+hipError_t rows_mt(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
+    switch (sh.mt) {
+    case 1: return rows_go<KIND, WP, XP, 1, FORM>(sh, a, s);
+    case 4: return rows_go<KIND, WP, XP, 4, FORM>(sh, a, s);
+    case 8:
+        if constexpr (XP == 1) return rows_go<KIND, WP, XP, 8, FORM>(sh, a, s);
+        break;
+    }
+    return hipErrorInvalidValue;
+}
+
+template <int KIND, int WP, int XP>
+hipError_t rows_form(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
+    switch (sh.form) {
+    case ROWS_PLAIN: return rows_mt<KIND, WP, XP, ROWS_PLAIN>(sh, a, s);
+    case ROWS_GLU: return rows_mt<KIND, WP, XP, ROWS_GLU>(sh, a, s);
+    case ROWS_LORA: return rows_mt<KIND, WP, XP, ROWS_LORA>(sh, a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+// Binary weights are exact in one plane.
+template <int KIND>
+hipError_t launch_rows_kind(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
+    constexpr int W2 = KIND == HK_BIN ? 1 : 2;
+    if (sh.xp == 2) return rows_form<KIND, W2, 2>(sh, a, s);
+    if (sh.wp == 2) return rows_form<KIND, W2, 1>(sh, a, s);
+    return rows_form<KIND, 1, 1>(sh, a, s);
+}
+
+}  // namespace hk

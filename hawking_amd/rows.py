@@ -1,0 +1,203 @@
+"""Products of many rows with packed organs: the routed experts of a prefill
+or of a decode step of many requests, and low-rank adapters of many requests
+beside a shared projection.
+
+Rows are grouped by an id (hk_group_rows), multiplied with the organ of their
+group (hk_gemm_grouped, hk_gemm_grouped_swiglu, hk_gemm_lora) and, for routed
+experts, summed per token (hk_combine_rows).  No call copies to the host or
+synchronises; every object holds the workspace of its calls, so one object is
+not to be used on two streams at once.
+
+A routed block of a batch, with ids and weights [tokens, top_k] on the device
+(a router's output):
+
+    plan = RowGroups(ctx, tokens * top_k, n_experts)
+    plan.build(ids)
+    gate_up(x, plan, act, gather=True, per_row=top_k)   # GroupedSwiGlu
+    down(act, plan, out)                                # GroupedGemm
+    combine_rows(ctx, out, plan.pos, weights, top_k, h, base=h)
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from ._lib import HK_T_BF16, HK_T_F16, HK_T_F32, RowsSrc
+from .organs import OrganSet, PackedOrgan
+from .runtime import Context, DeviceArray
+
+ROW_TYPES = {"f32": HK_T_F32, "bf16": HK_T_BF16, "f16": HK_T_F16}
+
+
+def _row_type(dtype: str) -> int:
+    if dtype not in ROW_TYPES:
+        raise ValueError(f"rows are f32, bf16 or f16, not {dtype!r}")
+    return ROW_TYPES[dtype]
+
+
+def _dp(a):
+    """Device pointer of an object with a .ptr, a raw c_void_p, or None."""
+    return getattr(a, "ptr", a)
+
+
+class Rows:
+    """n rows of `cols` elements of a device buffer (a DeviceArray, an object
+    with a .ptr, or a c_void_p), `stride` elements apart."""
+
+    def __init__(self, buf, n: int, cols: int, dtype: str = "f32", stride: int | None = None):
+        self.buf, self.n, self.cols, self.dtype = buf, int(n), int(cols), dtype
+        self.stride = self.cols if stride is None else int(stride)
+        self.src = RowsSrc(_dp(buf), _row_type(dtype), self.n, self.stride)
+        self.ref = C.byref(self.src)
+
+    @classmethod
+    def of(cls, arr: DeviceArray, dtype: str | None = None) -> "Rows":
+        """The rows of a two-dimensional DeviceArray (bf16 arrays hold uint16 bits: name the type)."""
+        n, cols = arr.shape
+        if dtype is None:
+            dtype = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16"}[arr.dtype]
+        return cls(arr, n, cols, dtype)
+
+
+class RowGroups:
+    """n ids grouped over n_groups (hk_group_rows): offsets [n_groups + 1],
+    order [n] and pos [n] on the device, and the call's workspace.  Buffers
+    that the caller owns may be given."""
+
+    def __init__(self, ctx: Context, n: int, n_groups: int, offsets=None, order=None, pos=None):
+        self.ctx, self.n, self.n_groups = ctx, int(n), int(n_groups)
+        self.offsets = ctx.empty(self.n_groups + 1, np.int32) if offsets is None else offsets
+        self.order = ctx.empty(self.n, np.int32) if order is None else order
+        self.pos = ctx.empty(self.n, np.int32) if pos is None else pos
+        self.ws_bytes = int(ctx.L.hk_group_rows_workspace(self.n, self.n_groups))
+        self.ws = ctx.empty(self.ws_bytes, np.uint8) if self.ws_bytes else None
+
+    def build(self, ids, stream=None) -> "RowGroups":
+        self.ctx.call("hk_group_rows", _dp(ids), self.n, self.n_groups, _dp(self.offsets), _dp(self.order), _dp(self.pos),
+                      _dp(self.ws), self.ws_bytes, stream if stream is not None else self.ctx.stream)
+        return self
+
+
+class _Product:
+    """Workspace and shape checks of a product with fixed organs and types."""
+
+    def _bind(self, ctx: Context, rows: int, cols: int, x_type: str, y_type: str):
+        self.ctx, self.rows, self.cols = ctx, rows, cols
+        self.x_type, self.y_type = x_type, y_type
+        _row_type(x_type), _row_type(y_type)
+        self.ws, self.ws_bytes, self._fits = None, 0, None
+
+    def _check(self, x: Rows, y: Rows, size) -> None:
+        if x.dtype != self.x_type or y.dtype != self.y_type:
+            raise ValueError(f"rows of {x.dtype} -> {y.dtype} given to a product of {self.x_type} -> {self.y_type}")
+        if x.cols != self.cols or y.cols != self.rows:
+            raise ValueError(f"rows of {x.cols} -> {y.cols} do not fit organs of {self.rows} x {self.cols}")
+        if self._fits != (x.n, y.n):
+            need = int(size(x.n, y.n))
+            if need > self.ws_bytes:
+                # calls of the old workspace may be in flight
+                self.ctx.device_synchronize()
+                self.ws = self.ctx.empty(need, np.uint8)
+                self.ws_bytes = need
+            self._fits = (x.n, y.n)
+
+
+class GroupedGemm(_Product):
+    """y_p = W_g x_p over the organs of a set (hk_gemm_grouped), for rows of
+    x_type -> y_type; the workspace is made for max_rows rows of x, gathered
+    or in grouped order, and grows (synchronising) where a call needs more."""
+
+    def __init__(self, ctx: Context, organs: OrganSet, max_rows: int, x_type: str = "f32", y_type: str = "f32"):
+        self.organs = organs
+        self._bind(ctx, organs.rows, organs.cols, x_type, y_type)
+        self._reserve(max_rows)
+
+    def _size(self, x_rows: int, n: int) -> int:
+        return self.ctx.L.hk_gemm_grouped_workspace(self.organs.h, x_rows, ROW_TYPES[self.x_type], n, ROW_TYPES[self.y_type])
+
+    def _reserve(self, max_rows: int) -> None:
+        self.ws_bytes = int(self._size(max_rows, max_rows))
+        self.ws = self.ctx.empty(self.ws_bytes, np.uint8)
+
+    def __call__(self, x: Rows, groups: RowGroups, y: Rows, gather: bool = False, per_row: int = 1, stream=None) -> None:
+        """gather: position p reads x row order[p] / per_row, else row p."""
+        self._check(x, y, self._size)
+        self.ctx.call("hk_gemm_grouped", self.organs.h, x.ref, _dp(groups.order) if gather else None, per_row,
+                      _dp(groups.offsets), y.ref, self.ws.ptr, self.ws_bytes,
+                      stream if stream is not None else self.ctx.stream)
+
+
+class GroupedSwiGlu(GroupedGemm):
+    """y_p = silu(G_g x_p) * (U_g x_p) over two sets (hk_gemm_grouped_swiglu)."""
+
+    def __init__(self, ctx: Context, gate: OrganSet, up: OrganSet, max_rows: int, x_type: str = "f32", y_type: str = "f32"):
+        if (gate.rows, gate.cols) != (up.rows, up.cols):
+            raise ValueError("the gate and up sets must have one shape")
+        self.up = up
+        super().__init__(ctx, gate, max_rows, x_type, y_type)
+
+    def __call__(self, x: Rows, groups: RowGroups, y: Rows, gather: bool = False, per_row: int = 1, stream=None) -> None:
+        self._check(x, y, self._size)
+        self.ctx.call("hk_gemm_grouped_swiglu", self.organs.h, self.up.h, x.ref, _dp(groups.order) if gather else None,
+                      per_row, _dp(groups.offsets), y.ref, self.ws.ptr, self.ws_bytes,
+                      stream if stream is not None else self.ctx.stream)
+
+
+def combine_rows(ctx: Context, x: Rows, pos, weights, per_row: int, y: Rows, base: Rows | None = None, stream=None) -> None:
+    """y_t = base_t + sum_r weights[t, r] x[pos[t, r]] (hk_combine_rows); base may be y."""
+    if x.cols != y.cols or (base is not None and base.cols != y.cols):
+        raise ValueError("x, base and y must have rows of one length")
+    ctx.call("hk_combine_rows", x.ref, _dp(pos), _dp(weights), per_row, y.cols, base.ref if base is not None else None,
+             y.ref, stream if stream is not None else ctx.stream)
+
+
+class LoraBank:
+    """n_slots adapters of rank up to max_rank beside one projection
+    (hk_lora_bank_create), laid out for that organ's kind and shape."""
+
+    def __init__(self, ctx: Context, organ: PackedOrgan, n_slots: int, max_rank: int):
+        self.ctx, self.rows, self.cols = ctx, organ.rows, organ.cols
+        self.n_slots, self.max_rank = int(n_slots), int(max_rank)
+        h = C.c_void_p()
+        ctx.call("hk_lora_bank_create", organ.h, self.n_slots, self.max_rank, C.byref(h))
+        self.h = h
+
+    def set(self, slot: int, rank: int, a, b, dtype: str = "bf16", scale: float = 1.0, stream=None) -> None:
+        """Adapter scale * B A from device arrays a [rank, cols] and b [rows, rank]; rank 0 empties the slot."""
+        self.ctx.call("hk_lora_bank_set", self.h, slot, rank, _dp(a), _dp(b), _row_type(dtype), scale,
+                      stream if stream is not None else self.ctx.stream)
+
+    def free(self):
+        if getattr(self, "h", None) and self.h.value and self.ctx.h:
+            self.ctx.L.hk_lora_bank_free(self.ctx.h, self.h)
+        self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class LoraGemm(_Product):
+    """y_i = W x_i + scale_s B_s (A_s x_i), s the adapter of row i
+    (hk_gemm_lora); groups: RowGroups over the rows' adapter ids and the
+    bank's slots."""
+
+    def __init__(self, ctx: Context, organ: PackedOrgan, bank: LoraBank, max_rows: int, x_type: str = "f32",
+                 y_type: str = "f32"):
+        self.organ, self.bank = organ, bank
+        self._bind(ctx, organ.rows, organ.cols, x_type, y_type)
+        self.ws_bytes = int(self._size(max_rows, max_rows))
+        self.ws = ctx.empty(self.ws_bytes, np.uint8)
+
+    def _size(self, x_rows: int, n: int) -> int:
+        return self.ctx.L.hk_gemm_lora_workspace(self.bank.h, max(x_rows, n), ROW_TYPES[self.x_type], ROW_TYPES[self.y_type])
+
+    def __call__(self, x: Rows, groups: RowGroups, y: Rows, in_order: bool = False, stream=None) -> None:
+        """in_order: the rows are in grouped order already."""
+        self._check(x, y, self._size)
+        self.ctx.call("hk_gemm_lora", self.organ.h, self.bank.h, x.ref, None if in_order else _dp(groups.order),
+                      _dp(groups.offsets), y.ref, self.ws.ptr, self.ws_bytes,
+                      stream if stream is not None else self.ctx.stream)

@@ -630,6 +630,114 @@ int hk_moe15_decode_layer(hk_ctx* ctx, hk_moe15_layer* layer, const float* h, fl
 int hk_moe15_decode_stack(hk_ctx* ctx, hk_moe15_layer* const* layers, uint32_t n_layers, const float* h, float* out,
                           int32_t* ids, float* weights, hk_stream stream);
 
+/* ------------------------------------------------- products of many rows
+ * Rows of a batch (tokens of a prefill, requests of a decode step) grouped by
+ * an id -- an expert, an adapter -- and multiplied with the packed matrix of
+ * their group.  No reference counterpart as calls of their own (the reference
+ * runs its routed experts one token at a time, run_qwen80_routed_expert_table
+ * model/qwen80_device_expert_table.rs:1204-1247, and a batch through
+ * moe_grouped_gemm_q4, shaders/moe.metal:333-).  A routed block of a batch is
+ * hk_router_* -> hk_group_rows -> hk_gemm_grouped_swiglu -> hk_gemm_grouped ->
+ * hk_combine_rows; no call copies to the host or synchronises.
+ *
+ * Numerics: sums in f32; y f32 or f16: within 2e-5 relative L2 of the exact
+ * product (weights exact, bf16 and f16 x exact, f32 x to 22 bits); y bf16:
+ * each weight code * scale is also rounded to 11 bits, which bf16's rounding
+ * of y exceeds eightfold.  A row of x that holds a non-finite value gives NaN
+ * in its rows of y and latches HK_E_NONFINITE's device bit
+ * (hk_check_device_status), as does any result that is not finite before it
+ * is rounded to y's type; |code * scale| must be below 65520 (an f16), else
+ * the results are not finite.  Results do not depend on the other rows of the
+ * batch's values, and equal calls give equal bits. */
+
+/* Element types of rows. */
+#define HK_T_F32 0
+#define HK_T_BF16 1
+#define HK_T_F16 2
+
+/* n rows in device memory, row i at data + i * stride elements.  data needs
+ * the alignment of an element; 16-byte aligned data with a stride that is a
+ * multiple of 8 elements is fastest. */
+typedef struct hk_rows {
+    void* data;
+    int32_t type;   /* HK_T_* */
+    uint32_t n;
+    size_t stride;  /* elements, >= the row length (ignored for n <= 1) */
+} hk_rows;
+
+/* Stable grouping of n ids (device int32) over n_groups groups:
+ *   offsets[n_groups + 1]  group g is positions [offsets[g], offsets[g + 1])
+ *   order[n]               order[p] = the index whose id is at position p;
+ *                          indexes keep their order inside a group, and ids
+ *                          outside [0, n_groups) (padding) come last, from
+ *                          offsets[n_groups] on
+ *   pos[n]                 the position of index i, -1 for an id outside
+ * All device int32; ids must not overlap the outputs.  ws: device memory of
+ * hk_group_rows_workspace(n, n_groups) bytes (0 for few ids: ws may be NULL),
+ * written by the call.  n may be 0 (offsets are written).  Limits
+ * (HK_E_UNSUPPORTED beyond): n < 2^31, 1 <= n_groups <= 8192. */
+size_t hk_group_rows_workspace(uint32_t n, uint32_t n_groups);
+int hk_group_rows(hk_ctx* ctx, const int32_t* ids, uint32_t n, uint32_t n_groups, int32_t* offsets, int32_t* order,
+                  int32_t* pos, void* ws, size_t ws_bytes, hk_stream stream);
+
+/* y_p = W_g x_r for every position p of every group g of the set's organs
+ * (offsets[set organs + 1], device, as hk_group_rows writes them):
+ *   r = order[p] / per_row   (order from hk_group_rows over ids [x->n][per_row]:
+ *                             a token's row of x, gathered), or
+ *   r = p                    (order NULL: x is in grouped order already)
+ * x: rows of the organs' cols, y: n rows of the organs' rows, n = y->n the
+ * number of positions (offsets[last] <= n).  Rows of y from offsets[last] on
+ * are not written.  A position whose r is not below x->n gives NaN and latches
+ * HK_E_ROUTE's device bit; offsets outside [0, n] are clamped.  x and y must
+ * not overlap.  Every kind but HK_F32 and HGRAVR02 (HK_E_UNSUPPORTED).  The
+ * weights of a group are read once for every 128 of its rows (64 or 16 where
+ * groups are small).  ws: 256-byte aligned device memory of
+ * hk_gemm_grouped_workspace bytes that no other call uses meanwhile (calls on
+ * two streams, or two captured graphs that may run at once, need one each). */
+size_t hk_gemm_grouped_workspace(const hk_organ_set* set, uint32_t x_rows, int32_t x_type, uint32_t n, int32_t y_type);
+int hk_gemm_grouped(hk_ctx* ctx, const hk_organ_set* set, const hk_rows* x, const int32_t* order, uint32_t per_row,
+                    const int32_t* offsets, const hk_rows* y, void* ws, size_t ws_bytes, hk_stream stream);
+/* y_p = silu(G_g x_r) * (U_g x_r), silu(v) = v / (1 + e^-v), with the gate and
+ * the up organs of two sets of one kind and shape, in one pass over x; the
+ * rest (and the workspace) as hk_gemm_grouped. */
+int hk_gemm_grouped_swiglu(hk_ctx* ctx, const hk_organ_set* gate, const hk_organ_set* up, const hk_rows* x,
+                           const int32_t* order, uint32_t per_row, const int32_t* offsets, const hk_rows* y, void* ws,
+                           size_t ws_bytes, hk_stream stream);
+
+/* y_t = base_t + sum over r < per_row, ascending, of weights[t, r] x[pos[t, r]],
+ * in f32 with one rounding: the end of a routed block (pos as hk_group_rows
+ * writes it for ids [y->n][per_row]; weights f32, both device).  Rows of
+ * `cols` elements.  A pos outside [0, x->n) adds nothing (a dropped route).
+ * base may be NULL (zero) or y itself; x must not overlap y. */
+int hk_combine_rows(hk_ctx* ctx, const hk_rows* x, const int32_t* pos, const float* weights, uint32_t per_row,
+                    uint32_t cols, const hk_rows* base, const hk_rows* y, hk_stream stream);
+
+/* Low-rank adapters of one packed projection (rows x cols), many at once.
+ * A bank holds n_slots adapters of rank up to max_rank <= 256, laid out for
+ * the projection's kind and shape (which it keeps; the organ itself is not
+ * referenced after the call). */
+typedef struct hk_lora_bank hk_lora_bank;
+int hk_lora_bank_create(hk_ctx* ctx, const hk_organ* organ, uint32_t n_slots, uint32_t max_rank, hk_lora_bank** out);
+int hk_lora_bank_free(hk_ctx* ctx, hk_lora_bank* bank);
+/* Adapter `slot` = scale * B A, a [rank x cols] and b [rows x rank] row-major
+ * device arrays of `type` (HK_T_BF16 or HK_T_F16; both are kept exactly down to
+ * 2^-28 of the matrix's largest value).  rank 0 empties the slot (a, b NULL).
+ * Stream-ordered: a slot may be replaced between products on one stream.  A
+ * non-finite value latches HK_E_NONFINITE's device bit and makes the slot's
+ * rows NaN. */
+int hk_lora_bank_set(hk_ctx* ctx, hk_lora_bank* bank, uint32_t slot, uint32_t rank, const void* a, const void* b,
+                     int32_t type, float scale, hk_stream stream);
+/* y_i = W x_i + scale_s B_s (A_s x_i), s the adapter of row i: hk_group_rows
+ * over the rows' adapter ids with n_groups = the bank's n_slots gives offsets
+ * and order (rows with an id outside, say -1, have no adapter: y_i = W x_i);
+ * order NULL: the rows are in grouped order already.  x->n = y->n rows; x and
+ * y in the batch's own order, not overlapping.  order must be a permutation
+ * (an index outside the rows is dropped and latches HK_E_ROUTE's device bit).
+ * ws as in hk_gemm_grouped, hk_gemm_lora_workspace bytes. */
+size_t hk_gemm_lora_workspace(const hk_lora_bank* bank, uint32_t n, int32_t x_type, int32_t y_type);
+int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_bank* bank, const hk_rows* x, const int32_t* order,
+                 const int32_t* offsets, const hk_rows* y, void* ws, size_t ws_bytes, hk_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,542 @@
+"""Row products against 64-bit evaluations of their definitions: grouping,
+ragged grouped products (plain and SwiGLU), the weighted sum of a token's
+rows, and the calls in a chain, eager and captured.  Bounds are those of
+hk_rowsutil, which counts the roundings; y f32 is also held to the 2e-5
+relative L2 of the documentation."""
+import ctypes as C
+import sys
+
+import numpy as np
+import pytest
+
+from tests import hk_rowsutil as R
+from tests import hk_testutil as U
+
+pytestmark = pytest.mark.gpu
+TYPES = [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32"), ("f16", "f16"), ("f32", "bf16")]
+
+
+def say(*a):
+    print("[gpu-case]", *a, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from hawking_amd.runtime import Context
+    return Context(0)
+
+
+# ---------------------------------------------------------------- grouping
+
+def _ids(rng, n, groups, how):
+    if how == "one":
+        return np.full(n, groups - 1, np.int32)
+    if how == "none":
+        return np.full(n, -1, np.int32)
+    if how == "skew":
+        return np.minimum(rng.geometric(0.2, n) - 1, groups).astype(np.int32)
+    ids = rng.integers(-2, groups + 2, n).astype(np.int32)
+    ids[rng.random(n) < 0.02] = np.iinfo(np.int32).min
+    ids[rng.random(n) < 0.02] = np.iinfo(np.int32).max
+    return ids
+
+
+# both launch forms: up to 2^22 id reads (n times n_groups + 1) a workgroup a
+# group, beyond that counts and places, with 16 waves a part up to 2048 groups and 4 beyond
+GROUPS = [(0, 1), (1, 1), (1, 8192), (5, 2), (63, 3), (64, 255), (65, 256), (255, 512), (257, 7), (512, 256), (4097, 512),
+          (8175, 512), (8176, 512), (8193, 512), (4097, 1024), (2049, 2048), (100000, 100), (327680, 512), (513, 8192), (4096, 2049),
+          (30001, 8192), (1 << 20, 4), (1 << 20, 3), (65537, 64)]
+
+
+@pytest.mark.parametrize("how", ["mixed", "one", "none", "skew"])
+@pytest.mark.parametrize("n,groups", GROUPS)
+def test_group_rows(ctx, n, groups, how):
+    from hawking_amd.rows import RowGroups
+    say("group", n, groups, how)
+    rng = np.random.default_rng(n * 31 + groups)
+    ids = _ids(rng, n, groups, how)
+    plan = RowGroups(ctx, n, groups).build(ctx.to_device(ids))
+    offsets, order, pos = R.group_oracle(ids, groups)
+    assert np.array_equal(plan.offsets.download(), offsets)
+    assert np.array_equal(plan.order.download()[:n], order)
+    assert np.array_equal(plan.pos.download()[:n], pos)
+
+
+def test_group_rows_refusals(ctx):
+    from hawking_amd._lib import HK_E_INVALID_ARG, HK_E_UNSUPPORTED, HawkingError
+    from hawking_amd.rows import RowGroups
+    d = ctx.to_device(np.zeros(16384, np.int32))
+    for groups, code in ((0, HK_E_UNSUPPORTED), (8193, HK_E_UNSUPPORTED)):
+        with pytest.raises(HawkingError) as e:
+            ctx.call("hk_group_rows", d.ptr, 4, groups, d.offset(100), d.offset(9000), d.offset(9100), None, 0, None)
+        assert e.value.code == code
+    plan = RowGroups(ctx, 16384, 512)
+    assert plan.ws_bytes > 0
+    with pytest.raises(HawkingError) as e:
+        ctx.call("hk_group_rows", d.ptr, 16384, 512, plan.offsets.ptr, plan.order.ptr, plan.pos.ptr, plan.ws.ptr,
+                 plan.ws_bytes - 4, None)
+    assert e.value.code == HK_E_INVALID_ARG
+
+
+# ---------------------------------------------------------------- grouped products
+
+def _plan(ctx, counts, extra=0):
+    """A plan whose groups have `counts` rows, and `extra` positions behind the last group."""
+    from hawking_amd.rows import RowGroups
+    n = int(sum(counts)) + extra
+    off = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    return RowGroups(ctx, n, len(counts), offsets=ctx.to_device(off)), off, n
+
+
+def _check(got, exact, bound, y_type, what):
+    assert np.all(np.isfinite(got)), what
+    over = np.abs(got - exact) - R.rounded(bound, exact, y_type)
+    assert over.max(initial=-1.0) <= 0.0, (what, float(over.max()), np.unravel_index(np.argmax(over), over.shape))
+    if y_type == "f32" and exact.size and np.linalg.norm(exact):
+        assert np.linalg.norm(got - exact) <= 2e-5 * np.linalg.norm(exact), what
+
+
+def _exact_grouped(xe, off, src, ws, x_type, y_type):
+    n, rows = len(src), ws[0].shape[0]
+    y, b = np.zeros((n, rows)), np.zeros((n, rows))
+    for g, w in enumerate(ws):
+        x = xe[src[off[g]:off[g + 1]]]
+        y[off[g]:off[g + 1]] = x @ w.T
+        b[off[g]:off[g + 1]] = R.product_bound(x, w, x_type, y_type)
+    return y, b
+
+
+COUNTS = {
+    # mean rows a group: up to 16 the split kernel, up to 64 the tile kernel with 64 rows, beyond with 128 (64 for f32 -> f32)
+    "few": [0, 1, 2, 15, 16, 17, 0, 0, 33, 1],
+    "mid": [20, 0, 64, 65, 1, 130],
+    "many": [129, 0, 257, 1, 300],
+    "lone": [1],
+}
+SHAPES = {
+    # odd rows, one row tile, one or several stages, a last step that is not full
+    "q4": [(17, 32), (60, 160), (256, 128), (300, 1184)],
+    "q8": [(17, 64), (100, 192), (320, 1088)],
+    "u3": [(1, 32), (60, 160), (270, 1056)],
+    "bin": [(17, 128), (100, 640), (257, 1152)],
+    "mixed": [(17, 128), (100, 640), (257, 1152)],
+}
+
+
+@pytest.mark.parametrize("x_type,y_type", TYPES)
+@pytest.mark.parametrize("counts", sorted(COUNTS))
+@pytest.mark.parametrize("kind", sorted(SHAPES))
+def test_grouped_product(ctx, oracle, kind, counts, x_type, y_type):
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    for rows, cols in SHAPES[kind]:
+        say("product", kind, rows, cols, counts, x_type, y_type)
+        cs = COUNTS[counts]
+        rng = np.random.default_rng(rows * cols + len(cs))
+        made = [R.make_organ(ctx, oracle, kind, rows, cols, rows * 7 + g) for g in range(len(cs))]
+        plan, off, n = _plan(ctx, cs, extra=3)
+        x, xb, xe = R.rows_on(ctx, rng.standard_normal((n, cols)), x_type)
+        y, yb, _ = R.rows_on(ctx, np.full((n, rows), 5.0), y_type, fill=5.0)
+        ctx.device_status()
+        GroupedGemm(ctx, OrganSet(ctx, [m[0] for m in made]), n, x_type, y_type)(x, plan, y)
+        got, rest = R.read_rows(yb, y)
+        exact, bound = _exact_grouped(xe[:off[-1]], off, np.arange(off[-1]), [m[1] for m in made], x_type, y_type)
+        _check(got[:off[-1]], exact, bound, y_type, (kind, rows, cols, counts))
+        assert np.all(got[off[-1]:] == 5.0) and np.all(rest == 5.0)  # rows behind the last group, and what is not a row
+        assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("group", [64, 128])
+def test_grouped_product_q4_groups(ctx, oracle, group):
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    say("product q4 group", group)
+    cs, rows, cols = [3, 70, 9], 48, 640
+    made = [R.make_organ(ctx, oracle, "q4", rows, cols, 900 + g, group=group) for g in range(3)]
+    plan, off, n = _plan(ctx, cs)
+    x, _, xe = R.rows_on(ctx, np.random.default_rng(group).standard_normal((n, cols)), "bf16")
+    y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+    GroupedGemm(ctx, OrganSet(ctx, [m[0] for m in made]), n, "bf16", "f32")(x, plan, y)
+    exact, bound = _exact_grouped(xe, off, np.arange(n), [m[1] for m in made], "bf16", "f32")
+    _check(R.read_rows(yb, y)[0], exact, bound, "f32", group)
+
+
+@pytest.mark.parametrize("x_type,y_type", TYPES)
+@pytest.mark.parametrize("stride,lead", [(0, 0), (1, 0), (3, 1), (8, 4)])
+def test_strides_and_alignment(ctx, oracle, x_type, y_type, stride, lead):
+    """Rows further apart than they are long, data off every vector alignment:
+    the same bits as packed rows, nothing written between the rows."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    say("strides", x_type, y_type, stride, lead)
+    cs, rows, cols = [5, 0, 40], 70, 256
+    rng = np.random.default_rng(5)
+    made = [R.make_organ(ctx, oracle, "q4", rows, cols, 950 + g) for g in range(3)]
+    s = OrganSet(ctx, [m[0] for m in made])
+    plan, off, n = _plan(ctx, cs)
+    v = rng.standard_normal((n, cols))
+    gemm = GroupedGemm(ctx, s, n, x_type, y_type)
+    x0, _, _ = R.rows_on(ctx, v, x_type)
+    y0, yb0, _ = R.rows_on(ctx, np.zeros((n, rows)), y_type)
+    gemm(x0, plan, y0)
+    x, _, _ = R.rows_on(ctx, v, x_type, stride=cols + stride, lead=lead, fill=np.nan)
+    y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), y_type, stride=rows + stride, lead=lead, fill=7.0)
+    gemm(x, plan, y)
+    got, rest = R.read_rows(yb, y)
+    assert np.array_equal(got, R.read_rows(yb0, y0)[0])
+    assert np.all(rest == 7.0)
+
+
+@pytest.mark.parametrize("kind,rows,cols", [("q4", 48, 320), ("mixed", 40, 512), ("q8", 33, 128)])
+@pytest.mark.parametrize("tokens,per_row,groups", [(1, 1, 4), (1, 10, 64), (7, 3, 16), (64, 8, 32), (300, 4, 6), (500, 2, 3)])
+@pytest.mark.parametrize("x_type,y_type", TYPES[:3])
+def test_swiglu_gathered(ctx, oracle, kind, rows, cols, tokens, per_row, groups, x_type, y_type):
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedSwiGlu, RowGroups
+    say("swiglu", kind, rows, cols, tokens, per_row, groups, x_type, y_type)
+    rng = np.random.default_rng(tokens * 100 + per_row)
+    ids = rng.integers(-1, groups, (tokens, per_row)).astype(np.int32).reshape(-1)
+    made = [(R.make_organ(ctx, oracle, kind, rows, cols, 2000 + 2 * g), R.make_organ(ctx, oracle, kind, rows, cols, 2001 + 2 * g))
+            for g in range(groups)]
+    plan = RowGroups(ctx, ids.size, groups).build(ctx.to_device(ids))
+    off, order, _ = R.group_oracle(ids, groups)
+    x, _, xe = R.rows_on(ctx, rng.standard_normal((tokens, cols)) * 2, x_type)
+    y, yb, _ = R.rows_on(ctx, np.full((ids.size, rows), 5.0), y_type)
+    GroupedSwiGlu(ctx, OrganSet(ctx, [m[0][0] for m in made]), OrganSet(ctx, [m[1][0] for m in made]), tokens, x_type, y_type)(
+        x, plan, y, gather=True, per_row=per_row)
+    src = order[:off[-1]] // per_row
+    g, bg = _exact_grouped(xe, off, src, [m[0][1] for m in made], x_type, y_type)
+    u, bu = _exact_grouped(xe, off, src, [m[1][1] for m in made], x_type, y_type)
+    got = R.read_rows(yb, y)[0]
+    exact = R.silu(g) * u
+    assert np.all(np.abs(got[:off[-1]] - exact) <= R.rounded(R.swiglu_bound(g, bg, u, bu), exact, y_type))
+    assert np.all(got[off[-1]:] == 5.0)
+
+
+def test_rows_do_not_depend_on_each_other(ctx, oracle):
+    """A row's bits are the same alone in its group and among others of one launch shape."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    rows, cols = 64, 384
+    w = R.make_organ(ctx, oracle, "q4", rows, cols, 3000)[0]
+    v = np.random.default_rng(1).standard_normal((16, cols))
+    for n in (1, 16):
+        plan, _, _ = _plan(ctx, [n])
+        x, _, _ = R.rows_on(ctx, v[:n], "f32")
+        y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+        GroupedGemm(ctx, OrganSet(ctx, [w]), n, "f32", "f32")(x, plan, y)
+        first = R.read_rows(yb, y)[0][0] if n == 1 else first
+        last = R.read_rows(yb, y)[0]
+    assert np.array_equal(first, last[0])
+
+
+@pytest.mark.parametrize("x_type", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 1.0, 1e4, 1e30])
+def test_magnitudes(ctx, oracle, x_type, scale):
+    """Rows of very different magnitude side by side, an all-zero row, and one
+    element far above the rest of its row."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    if x_type == "f16" and not 1e-5 < scale < 1e5:
+        scale = 1e-4 if scale < 1 else 1e3
+    say("magnitudes", x_type, scale)
+    rows, cols = 40, 256
+    w, we = R.make_organ(ctx, oracle, "q8", rows, cols, 3100)
+    v = np.random.default_rng(2).standard_normal((6, cols)) * scale
+    v[1] = 0.0
+    v[2] *= 1e-3
+    v[3, 7] *= 1e4 if x_type != "f16" else 10
+    v[4] = 0.0
+    v[4, cols - 1] = scale
+    plan, off, n = _plan(ctx, [6])
+    x, _, xe = R.rows_on(ctx, v, x_type)
+    y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+    ctx.device_status()
+    GroupedGemm(ctx, OrganSet(ctx, [w]), n, x_type, "f32")(x, plan, y)
+    got = R.read_rows(yb, y)[0]
+    # (at 1e4 the f16 row of the large element holds an infinity: its results are NaN)
+    inf = ~np.isfinite(xe).all(1)
+    assert np.all(np.isnan(got[inf])) and ctx.device_status() == (1 if inf.any() else 0)
+    xe, got0 = xe[~inf], got[~inf]
+    exact = xe @ we.T
+    # (f32 results below 2^-126 are flushed or subnormal: one step of them)
+    assert np.all(np.abs(got0 - exact) <= R.rounded(R.product_bound(xe, we, x_type, "f32"), exact, "f32") + 2.0 ** -126)
+    assert np.all(got[1] == 0.0)
+
+
+@pytest.mark.parametrize("per", ["few", "many"])
+def test_nonfinite_rows(ctx, oracle, per):
+    """A NaN or an infinity makes its own row NaN, leaves the others, and latches the status."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    rows, cols, n = 32, 256, 8 if per == "few" else 200
+    w, we = R.make_organ(ctx, oracle, "q4", rows, cols, 3200)
+    v = np.random.default_rng(3).standard_normal((n, cols)).astype(np.float32)
+    v[1, 3], v[2, 200], v[5, 0] = np.nan, np.inf, -np.inf
+    plan, _, _ = _plan(ctx, [n])
+    for y_type in ("f32", "bf16"):
+        x, _, _ = R.rows_on(ctx, v, "f32")
+        y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), y_type)
+        ctx.device_status()
+        GroupedGemm(ctx, OrganSet(ctx, [w]), n, "f32", y_type)(x, plan, y)
+        got = R.read_rows(yb, y)[0]
+        assert np.all(np.isnan(got[[1, 2, 5]]))
+        ok = [i for i in range(n) if i not in (1, 2, 5)]
+        xe = v[ok].astype(np.float64)
+        exact = xe @ we.T
+        assert np.all(np.abs(got[ok] - exact) <= R.rounded(R.product_bound(xe, we, "f32", y_type), exact, y_type))
+        assert ctx.device_status() & 1
+
+
+@pytest.mark.parametrize("n", [9, 150])
+def test_wild_indexes_stay_inside(ctx, oracle, n):
+    """Source indexes outside x give NaN rows and latch the status; offsets
+    outside the positions are clamped (kernel bounds checks, no faults)."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm, RowGroups
+    say("wild indexes", n)
+    rows, cols = 32, 128
+    w, we = R.make_organ(ctx, oracle, "q4", rows, cols, 3300)
+    v = np.random.default_rng(4).standard_normal((n, cols))
+    order = np.arange(n, dtype=np.int32)
+    order[2], order[4] = n, -1
+    for off in ([0, n], [-5, n + 100], [0, 2 ** 31 - 1]):
+        plan = RowGroups(ctx, n, 1, offsets=ctx.to_device(np.array(off, np.int32)), order=ctx.to_device(order))
+        x, _, xe = R.rows_on(ctx, v, "bf16")
+        y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+        ctx.device_status()
+        GroupedGemm(ctx, OrganSet(ctx, [w]), n, "bf16", "f32")(x, plan, y, gather=True)
+        got = R.read_rows(yb, y)[0]
+        assert np.all(np.isnan(got[[2, 4]])) and ctx.device_status() & 2
+        ok = [i for i in range(n) if i not in (2, 4)]
+        assert np.linalg.norm(got[ok] - xe[ok] @ we.T) <= 2e-5 * np.linalg.norm(xe[ok] @ we.T)
+    # a range that ends before it begins, and one past the end, hold nothing
+    plan = RowGroups(ctx, n, 2, offsets=ctx.to_device(np.array([n, 0, -7], np.int32)))
+    y, yb, _ = R.rows_on(ctx, np.full((n, rows), 5.0), "f32")
+    GroupedGemm(ctx, OrganSet(ctx, [w, w]), n, "bf16", "f32")(x, plan, y)
+    assert np.all(R.read_rows(yb, y)[0] == 5.0)
+
+
+def test_product_refusals(ctx, oracle):
+    from hawking_amd._lib import HK_E_GEOMETRY, HK_E_INVALID_ARG, HK_E_UNSUPPORTED, HawkingError
+    from hawking_amd.organs import DenseF32Organ, OrganSet, SyntheticOrgan
+    from hawking_amd.rows import GroupedGemm, GroupedSwiGlu, Rows
+    w = R.make_organ(ctx, oracle, "q4", 32, 128, 3400)[0]
+    s = OrganSet(ctx, [w])
+    plan, _, _ = _plan(ctx, [4])
+    x, _, _ = R.rows_on(ctx, np.zeros((4, 128)), "f32")
+    y, _, _ = R.rows_on(ctx, np.zeros((4, 32)), "f32")
+    gemm = GroupedGemm(ctx, s, 4)
+
+    def code(fn):
+        with pytest.raises(HawkingError) as e:
+            fn()
+        return e.value.code
+
+    assert code(lambda: ctx.call("hk_gemm_grouped", s.h, x.ref, None, 1, plan.offsets.ptr, y.ref, gemm.ws.ptr,
+                                 gemm.ws_bytes - 1, None)) == HK_E_INVALID_ARG
+    assert code(lambda: ctx.call("hk_gemm_grouped", s.h, x.ref, plan.order.ptr, 0, plan.offsets.ptr, y.ref, gemm.ws.ptr,
+                                 gemm.ws_bytes, None)) == HK_E_INVALID_ARG
+    assert code(lambda: ctx.call("hk_gemm_grouped", None, x.ref, None, 1, plan.offsets.ptr, y.ref, gemm.ws.ptr,
+                                 gemm.ws_bytes, None)) == HK_E_INVALID_ARG
+    other = OrganSet(ctx, [R.make_organ(ctx, oracle, "q4", 32, 128, 3401, group=64)[0]])
+    assert code(lambda: ctx.call("hk_gemm_grouped_swiglu", s.h, other.h, x.ref, None, 1, plan.offsets.ptr, y.ref,
+                                 gemm.ws.ptr, gemm.ws_bytes, None)) == HK_E_GEOMETRY
+    for organ in (DenseF32Organ(ctx, np.zeros((32, 128), np.float32)),
+                  SyntheticOrgan(ctx, 6, 32, 128, R.key(oracle, 9), 0)):
+        odd = OrganSet(ctx, [organ])
+        assert code(lambda: GroupedGemm(ctx, odd, 4)(x, plan, y)) == HK_E_UNSUPPORTED
+    with pytest.raises(ValueError):
+        gemm(Rows(x.buf, 4, 128, "bf16"), plan, y)
+    with pytest.raises(ValueError):
+        gemm(Rows(x.buf, 4, 64, "f32"), plan, y)
+    with pytest.raises(ValueError):
+        GroupedSwiGlu(ctx, s, OrganSet(ctx, [R.make_organ(ctx, oracle, "q4", 16, 128, 3402)[0]]), 4)
+
+
+def test_no_rows(ctx, oracle):
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm, RowGroups
+    s = OrganSet(ctx, [R.make_organ(ctx, oracle, "bin", 32, 128, 3500)[0]])
+    plan = RowGroups(ctx, 0, 1).build(ctx.empty(1, np.int32))
+    x, _, _ = R.rows_on(ctx, np.zeros((0, 128)), "f32")
+    y, yb, _ = R.rows_on(ctx, np.zeros((0, 32)), "f32", fill=5.0)
+    GroupedGemm(ctx, s, 0)(x, plan, y)
+    ctx.synchronize()
+    assert np.all(yb.download()[:0] == 5.0) and np.array_equal(plan.offsets.download(), [0, 0])
+
+
+# ---------------------------------------------------------------- weighted sum
+
+@pytest.mark.parametrize("x_type,y_type", TYPES + [("bf16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("tokens,per_row,cols,stride,lead", [(1, 1, 1, 0, 0), (1, 10, 2048, 0, 0), (33, 8, 7168, 0, 0), (5, 3, 100, 0, 0),
+                                                             (17, 5, 257, 3, 1), (9, 6, 512, 8, 8), (300, 11, 64, 0, 0)])
+def test_combine_rows(ctx, x_type, y_type, tokens, per_row, cols, stride, lead):
+    from hawking_amd.rows import combine_rows
+    say("combine", x_type, y_type, tokens, per_row, cols)
+    rng = np.random.default_rng(tokens + cols)
+    n = tokens * per_row
+    x, _, xe = R.rows_on(ctx, rng.standard_normal((n, cols)), x_type, stride=cols + stride, lead=lead, fill=np.nan)
+    w = rng.random((tokens, per_row)).astype(np.float32)
+    pos = rng.permutation(n).astype(np.int32).reshape(tokens, per_row)
+    pos[rng.random((tokens, per_row)) < 0.2] = -1
+    pos[0, 0] = n  # outside: adds nothing
+    bv = rng.standard_normal((tokens, cols))
+    pd, wd = ctx.to_device(pos), ctx.to_device(w)
+    # 1 product and 1 sum a route and 1 for the base, each half a step of the terms' sum so far
+    exact, total = np.zeros((tokens, cols)), np.zeros((tokens, cols))
+    for r in range(per_row):
+        on = (pos[:, r] >= 0) & (pos[:, r] < n)
+        t = np.where(on[:, None], w[:, r].astype(np.float64)[:, None] * xe[np.where(on, pos[:, r], 0)], 0.0)
+        exact += t
+        total += np.abs(t)
+    for base in (None, "own", "y"):
+        y, yb, ye = R.rows_on(ctx, bv, y_type, stride=cols + stride, lead=lead, fill=7.0)
+        b, _, be = R.rows_on(ctx, bv, y_type)
+        combine_rows(ctx, x, pd, wd, per_row, y, base=None if base is None else (b if base == "own" else y))
+        got, rest = R.read_rows(yb, y)
+        add = be if base else 0.0
+        bound = (per_row + 2) * 2.0 ** -24 * (total + np.abs(add))
+        assert np.all(np.abs(got - (exact + add)) <= R.rounded(bound, exact + add, y_type)), base
+        assert np.all(rest == 7.0)
+
+
+# ---------------------------------------------------------------- chains
+
+def _block(ctx, oracle, tokens, top_k, experts, hidden, inter, kind, tag):
+    gate = [R.make_organ(ctx, oracle, kind, inter, hidden, tag + 3 * e) for e in range(experts)]
+    up = [R.make_organ(ctx, oracle, kind, inter, hidden, tag + 3 * e + 1) for e in range(experts)]
+    down = [R.make_organ(ctx, oracle, kind, hidden, inter, tag + 3 * e + 2) for e in range(experts)]
+    return gate, up, down
+
+
+@pytest.mark.parametrize("kind,tokens", [("q4", 1), ("q4", 5), ("mixed", 40), ("q4", 300)])
+def test_routed_block(ctx, oracle, kind, tokens):
+    """Router, grouping, SwiGLU, down projection and weighted sum as a prefill
+    runs them, f32 throughout, against the same block in 64 bits on the routes
+    the router chose; and against hk_moe_block's definition a token at a time."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm, GroupedSwiGlu, RowGroups, Rows, combine_rows
+    say("block", kind, tokens)
+    top_k, experts, hidden, inter = 4, 16, 256, 128
+    rng = np.random.default_rng(tokens)
+    gate, up, down = _block(ctx, oracle, tokens, top_k, experts, hidden, inter, kind, 5000)
+    sets = [OrganSet(ctx, [o for o, _ in p]) for p in (gate, up, down)]
+    h = rng.standard_normal((tokens, hidden)).astype(np.float32)
+    logits = ctx.to_device(rng.standard_normal((tokens, experts)).astype(np.float32))
+    ids, wts = ctx.empty((tokens, top_k), np.int32), ctx.empty((tokens, top_k))
+    hd, out = ctx.to_device(h), ctx.empty((tokens, hidden))
+    act, exp = ctx.empty((tokens * top_k, inter)), ctx.empty((tokens * top_k, hidden))
+    plan = RowGroups(ctx, tokens * top_k, experts)
+    gate_up = GroupedSwiGlu(ctx, sets[0], sets[1], tokens)
+    dn = GroupedGemm(ctx, sets[2], tokens * top_k)
+    ctx.call("hk_router_softmax_topk", logits.ptr, tokens, experts, top_k, 0.0, 1, ids.ptr, wts.ptr, ctx.stream)
+    plan.build(ids)
+    gate_up(Rows.of(hd), plan, Rows.of(act), gather=True, per_row=top_k)
+    dn(Rows.of(act), plan, Rows.of(exp))
+    combine_rows(ctx, Rows.of(exp), plan.pos, wts, top_k, Rows.of(out), base=Rows.of(hd))
+    got, i, w = out.download().astype(np.float64), ids.download(), wts.download().astype(np.float64)
+    want = h.astype(np.float64)
+    for t in range(tokens):
+        for r in range(top_k):
+            x = h[t].astype(np.float64)
+            want[t] += w[t, r] * (down[i[t, r]][1] @ (R.silu(gate[i[t, r]][1] @ x) * (up[i[t, r]][1] @ x)))
+    assert np.linalg.norm(got - want) <= 2e-5 * np.linalg.norm(want - h)
+
+
+class _Graph:
+    """A captured stream, replayed: straight calls of the HIP runtime the library has loaded."""
+
+    def __init__(self, ctx, stream):
+        self.hip, self.stream = C.CDLL("libamdhip64.so.7"), stream
+        self.graph, self.exe = C.c_void_p(), C.c_void_p()
+
+    def __enter__(self):
+        assert self.hip.hipStreamBeginCapture(self.stream, 2) == 0  # relaxed
+        return self
+
+    def __exit__(self, *a):
+        assert self.hip.hipStreamEndCapture(self.stream, C.byref(self.graph)) == 0
+        assert self.hip.hipGraphInstantiate(C.byref(self.exe), self.graph, None, None, C.c_size_t(0)) == 0
+
+    def replay(self):
+        assert self.hip.hipGraphLaunch(self.exe, self.stream) == 0
+        assert self.hip.hipStreamSynchronize(self.stream) == 0
+
+    def free(self):
+        self.hip.hipGraphExecDestroy(self.exe)
+        self.hip.hipGraphDestroy(self.graph)
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_captured_block(ctx, oracle, tokens):
+    """The block captured once and replayed on new routes and inputs, with eager
+    calls in between: every replay equals the eager result of its inputs."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm, GroupedSwiGlu, RowGroups, Rows, combine_rows
+    say("captured block", tokens)
+    top_k, experts, hidden, inter = 2, 8, 256, 128
+    rng = np.random.default_rng(tokens)
+    gate, up, down = _block(ctx, oracle, tokens, top_k, experts, hidden, inter, "q4", 6000)
+    sets = [OrganSet(ctx, [o for o, _ in p]) for p in (gate, up, down)]
+    stream = ctx.new_stream()
+
+    def make():
+        b = dict(h=ctx.empty((tokens, hidden)), ids=ctx.empty((tokens, top_k), np.int32), w=ctx.empty((tokens, top_k)),
+                 act=ctx.empty((tokens * top_k, inter)), exp=ctx.empty((tokens * top_k, hidden)), out=ctx.empty((tokens, hidden)),
+                 plan=RowGroups(ctx, tokens * top_k, experts), gu=GroupedSwiGlu(ctx, sets[0], sets[1], tokens),
+                 dn=GroupedGemm(ctx, sets[2], tokens * top_k))
+        b["x"], b["a"], b["e"], b["o"] = (Rows.of(b[k]) for k in ("h", "act", "exp", "out"))
+        return b
+
+    def calls(b):
+        b["plan"].build(b["ids"], stream=stream)
+        b["gu"](b["x"], b["plan"], b["a"], gather=True, per_row=top_k, stream=stream)
+        b["dn"](b["a"], b["plan"], b["e"], stream=stream)
+        combine_rows(ctx, b["e"], b["plan"].pos, b["w"], top_k, b["o"], base=b["x"], stream=stream)
+
+    cap, eager = make(), make()
+    cap["ids"].upload(np.zeros((tokens, top_k), np.int32), stream)
+    calls(cap)  # sizes the workspaces before the capture
+    eager["ids"].upload(np.zeros((tokens, top_k), np.int32), stream)
+    calls(eager)
+    ctx.synchronize(stream)
+    g = _Graph(ctx, stream)
+    with g:
+        calls(cap)
+    for k in range(4):
+        ids = rng.integers(-1, experts, (tokens, top_k)).astype(np.int32) if k else np.full((tokens, top_k), k, np.int32)
+        h, w = rng.standard_normal((tokens, hidden)).astype(np.float32), rng.random((tokens, top_k)).astype(np.float32)
+        for b in (cap, eager):
+            b["ids"].upload(ids, stream), b["h"].upload(h, stream), b["w"].upload(w, stream)
+        g.replay()
+        calls(eager)
+        ctx.synchronize(stream)
+        assert np.array_equal(cap["out"].download(stream), eager["out"].download(stream)), k
+    g.free()
+
+
+def test_two_streams(ctx, oracle):
+    """Two objects on two streams at once, each with its workspace: the bits of each alone."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    rows, cols = 512, 1024
+    s = OrganSet(ctx, [R.make_organ(ctx, oracle, "q4", rows, cols, 7000 + g)[0] for g in range(4)])
+    jobs = []
+    for k, counts in enumerate(([100, 3, 0, 90], [2, 2, 2, 2])):
+        plan, _, n = _plan(ctx, counts)
+        x, xb, _ = R.rows_on(ctx, np.random.default_rng(k).standard_normal((n, cols)), "bf16")
+        y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+        gemm = GroupedGemm(ctx, s, n, "bf16", "f32")
+        gemm(x, plan, y)
+        ctx.synchronize()
+        jobs.append((gemm, plan, x, xb, y, yb, yb.download(), ctx.new_stream()))
+    for gemm, plan, x, xb, y, yb, want, st in jobs:
+        yb.zero(st)
+    for _ in range(10):
+        for gemm, plan, x, xb, y, yb, want, st in jobs:
+            gemm(x, plan, y, stream=st)
+    ctx.device_synchronize()
+    for gemm, plan, x, xb, y, yb, want, st in jobs:
+        assert np.array_equal(yb.download(), want)
