@@ -99,6 +99,12 @@ __device__ __forceinline__ void rows_fetch(const OrganView& o, uint32_t T, uint3
 }
 
 __device__ __forceinline__ hk_f16x2 h2_bits(uint32_t v) { return __builtin_bit_cast(hk_f16x2, v); }
+// (v & mask) | magic as one v_and_or_b32: with both constants as literals the
+// compiler emits two instructions, so the second one is kept in a register.
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic) {
+    asm("" : "+v"(magic));
+    return (v & mask) | magic;
+}
 __device__ __forceinline__ hk_f16x2 h2_all(float v) { return hk_f16x2{(_Float16)v, (_Float16)v}; }
 __device__ __forceinline__ uint32_t both_halves(uint16_t s) { return (uint32_t)s | ((uint32_t)s << 16); }
 
@@ -124,10 +130,10 @@ __device__ __forceinline__ void rows_weights(const RowsW<KIND>& w, int a, int u,
     } else if constexpr (KIND == HK_Q4) {
         const uint32_t v = (&w.f[0].v[0].x)[u], v8 = v >> 8;
         const hk_f16x2 m8 = h2_all(-1032.0f), m72 = h2_all(-72.0f), r16 = h2_all(0.0625f);
-        c[0] = h2_bits((v & 0x000F000Fu) | 0x64006400u) + m8;
-        c[1] = __builtin_elementwise_fma(h2_bits((v & 0x00F000F0u) | 0x64006400u), r16, m72);
-        c[2] = h2_bits((v8 & 0x000F000Fu) | 0x64006400u) + m8;
-        c[3] = __builtin_elementwise_fma(h2_bits((v8 & 0x00F000F0u) | 0x64006400u), r16, m72);
+        c[0] = h2_bits(and_or(v, 0x000F000Fu, 0x64006400u)) + m8;
+        c[1] = __builtin_elementwise_fma(h2_bits(and_or(v, 0x00F000F0u, 0x64006400u)), r16, m72);
+        c[2] = h2_bits(and_or(v8, 0x000F000Fu, 0x64006400u)) + m8;
+        c[3] = __builtin_elementwise_fma(h2_bits(and_or(v8, 0x00F000F0u, 0x64006400u)), r16, m72);
         s2 = both_halves(w.f[0].s[0]);
     } else if constexpr (KIND == HK_U3) {
         const uint32_t lw = u < 2 ? w.f[0].lo[0].x : w.f[0].lo[0].y;
@@ -164,7 +170,7 @@ __device__ __forceinline__ void rows_weights(const RowsW<KIND>& w, int a, int u,
         for (int k = 0; k < 4; ++k) {
             const int i = 4 * u + k, r = ((i & ~1) + 30) & 31;
             const uint32_t x = (i & 1) ? o : e;
-            c[k] = __builtin_elementwise_fma(h2_bits((__builtin_amdgcn_alignbit(x, x, r) & mask) | 0x5C005C00u), A, B);
+            c[k] = __builtin_elementwise_fma(h2_bits(and_or(__builtin_amdgcn_alignbit(x, x, r), mask, 0x5C005C00u)), A, B);
         }
         s2 = both_halves(a < 2 ? w.f[0].s0[0] : w.f[0].s1[0]);
     }

@@ -7,6 +7,8 @@
 // consecutive rows of one position.
 #pragma once
 
+#include <type_traits>
+
 #include "hk_rows.h"
 
 namespace hk {
@@ -54,13 +56,24 @@ __device__ __forceinline__ void rows_store(const RowsArgs& a, uint32_t yr, uint3
     }
 }
 
+// f(0) .. f(N - 1) with the index a constant: sums indexed by it stay in
+// registers however large the body (an unroll pragma gives up on this one and
+// the sums of a 128-row tile then go through scratch memory).
+template <int N, class F>
+__device__ __forceinline__ void rows_each(F&& f) {
+    if constexpr (N > 0) {
+        rows_each<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+
 // The adapters' part: acc (units of 2^-exps) is moved to the units of the
 // position's mid row and B_s mid is added for every slot s with positions in
 // the tile [first, last); the other positions' mid counts as zero.  T: the
 // RT row tiles of this wave; exps: this lane's position of every 16, updated.
 template <int MT, int RT>
-__device__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane, int32_t* exps,
-                          hk_f32x4 (&acc)[MT][RT]) {
+__device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane,
+                                          int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
     const RowsLora& L = a.lora;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
     const size_t pitch = (size_t)L.kk_max * 64u * L.planes;
@@ -79,8 +92,7 @@ __device__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, cons
             const uint32_t lo = max(__builtin_amdgcn_readlane(o0, i), first), hi = min(__builtin_amdgcn_readlane(o1, i), last);
             const uint32_t kk = min((L.tab[s].rank + 31u) / 32u, L.kk_max);
             if (!kk) continue;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            rows_each<MT>([&](auto mt) {
                 const uint32_t p = first + 16u * mt + m;
                 if (p >= lo && p < hi) {
                     const int32_t g = L.mid_exps[p];
@@ -92,28 +104,30 @@ __device__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, cons
                         for (int j = 0; j < 4; ++j) acc[mt][r][j] = ldexpf(acc[mt][r][j], d);
                     exps[mt] = nan ? ROWS_EXP_BAD : g;
                 }
-            }
+            });
             for (uint32_t k = 0; k < kk; ++k) {
+                // opaque to the compiler: it would keep the MT rows' addresses in registers over the loop, and spill
+                uint32_t f = first;
+                asm volatile("" : "+s"(f));
                 hk_f16x8 w[RT];
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
                     w[r] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
                                                             L.b + (((size_t)s * a.n_row_tiles + T[r]) * L.kk_max + k) * 1024u + 16u * (uint32_t)lane)));
+                for (uint32_t pl = 0; pl < L.planes; ++pl)
+                    rows_each<MT>([&](auto mt) {
+                        const uint32_t t0 = f + 16u * mt;
+                        if (t0 < hi && t0 + 16u > lo) {  // uniform
+                            const uint32_t p = t0 + m;
+                            const bool mine = p >= lo && p < hi;
+                            uint4 v = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)(mine ? p : lo) * pitch +
+                                                                         ((size_t)pl * L.kk_max + k) * 64u + 16u * q));
+                            if (!mine) v = make_uint4(0u, 0u, 0u, 0u);
+                            const hk_f16x8 x = __builtin_bit_cast(hk_f16x8, v);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const uint32_t t0 = first + 16u * mt;
-                    if (t0 >= hi || t0 + 16u <= lo) continue;  // uniform
-                    const uint32_t p = t0 + m;
-                    const bool mine = p >= lo && p < hi;
-                    for (uint32_t pl = 0; pl < L.planes; ++pl) {
-                        uint4 v = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)(mine ? p : lo) * pitch +
-                                                                     ((size_t)pl * L.kk_max + k) * 64u + 16u * q));
-                        if (!mine) v = make_uint4(0u, 0u, 0u, 0u);
-                        const hk_f16x8 x = __builtin_bit_cast(hk_f16x8, v);
-#pragma unroll
-                        for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(w[r], x, acc[mt][r]);
-                    }
-                }
+                            for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(w[r], x, acc[mt][r]);
+                        }
+                    });
             }
         }
     }
@@ -158,24 +172,141 @@ __device__ __forceinline__ void rows_epilogue(const RowsArgs& a, uint32_t first,
 
 // ------------------------------------------------------------------ many rows a group: x through LDS
 
-// A workgroup of four waves: 16 MT positions x 16 row tiles (four a wave;
-// SwiGLU: two gate and two up).  Per stage (128 columns) the positions' image
-// is copied into one of two LDS buffers while the other is multiplied, with
-// one barrier a stage; each wave decodes its own weights in registers, so a
+// One wave's 64 lanes copy 64 x 16 bytes from global memory to LDS at `to`
+// (wave-uniform) + 16 lane without passing through registers.  Written as
+// assembly because the compiler would make every later LDS read wait for the
+// copy; it has no outputs, and rows_copied() waits for it before the barrier
+// that publishes the buffer.
+__device__ __forceinline__ void rows_copy16(const uint8_t* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void rows_copied() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// A tile of 16 MT positions x this workgroup's 16 row tiles.
+//
+// Four waves, four row tiles each (SwiGLU: two gate and two up).  Per stage
+// (128 columns) the positions' image is copied straight into one of two LDS
+// buffers while the other is multiplied, with one barrier a stage; each wave
+// decodes its own weights in registers, fetched a superstep ahead, so a
 // fragment of 16 rows x 32 columns serves MT products.  The 16-byte chunks of
 // a row are stored at chunk ^ (row % 16), so the 16 rows that a fragment read
 // touches lie in 16 different bank groups.
 template <int KIND, int WP, int XP, int MT, int FORM>
-__global__ void __launch_bounds__(256, 2) rows_tile_kernel(RowsArgs a) {
+__device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uint32_t first, uint32_t last, uint32_t block,
+                                          uint8_t* lds, const uint32_t* src, const int32_t* sexp) {
     constexpr int RT = 4, BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
     constexpr bool GLU = FORM == ROWS_GLU;
     constexpr uint32_t BUF = BM * 256u * XP;
-    extern __shared__ __align__(16) uint8_t lds[];  // 2 BUF
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
+
+    // x: this wave copies rows wave * 4 MT + 4 i + lane / 16, i < MT; lane l
+    // fills place l % 16 of its row
+    const size_t pitch16 = (size_t)a.stages * 16u * XP;  // image pitch in 16-byte chunks
+    uint32_t xo[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t row = wave * (4u * MT) + 4u * i + q;
+        xo[i] = (uint32_t)(src[row] * pitch16) + (m ^ (row & 15u));
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * (4u * MT) * 256u;
+    auto x_copy = [&](uint32_t s) {
+        const uint8_t* b = a.ws.img + (size_t)s * (256u * XP);
+        const uint32_t to = lds0 + (s & 1u) * BUF;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int p = 0; p < XP; ++p) rows_copy16(b + (size_t)xo[i] * 16u + 256u * p, to + p * (BM * 256u) + i * 1024u);
+    };
+
+    const OrganView o = a.organs[group];
+    const OrganView ou = GLU ? a.up[group] : o;
+    const uint32_t T0 = (block * 4u + wave) * (GLU ? RT / 2 : RT);
+    uint32_t T[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) T[r] = min(T0 + (uint32_t)(GLU ? r % (RT / 2) : r), a.n_row_tiles - 1u);
+    auto view = [&](int r) -> const OrganView& { return (GLU && r >= RT / 2) ? ou : o; };
+
+    const uint32_t n_super = a.stages / STG;
+    uint4 hdr[RT] = {};
+    auto heads = [&](uint32_t t) {
+        if constexpr (KIND == HK_MIXED) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) hdr[r] = ldg(view(r).hdr + (T[r] * view(r).steps + t));
+        }
+    };
+    RowsW<KIND> w[2][RT];
+    auto w_load = [&](uint32_t t, RowsW<KIND>(&x)[RT]) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) rows_fetch<KIND>(view(r), T[r], t, lane, hdr[r], x[r]);
+    };
+
+    hk_f32x4 acc[MT][RT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    x_copy(0);
+    heads(0);
+    w_load(0, w[0]);
+    heads(min(1u, n_super - 1u));
+    rows_copied();
+    __syncthreads();
+
+    auto super = [&](uint32_t t, RowsW<KIND>(&cur)[RT], RowsW<KIND>(&nxt)[RT]) {
+#pragma unroll
+        for (int st = 0; st < STG; ++st) {
+            const uint32_t s = t * STG + st;
+            // the other buffer was last read before the previous stage's barrier
+            x_copy(min(s + 1u, a.stages - 1u));
+            if (st == 0) {
+                w_load(min(t + 1u, n_super - 1u), nxt);
+                heads(min(t + 2u, n_super - 1u));
+            }
+            const uint8_t* b = lds + (s & 1u) * BUF + m * 256u;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint8_t* bu = b + (((4u * u + q) ^ m) * 16u);
+                hk_f16x8 x[MT][XP];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int p = 0; p < XP; ++p)
+                        x[mt][p] = *reinterpret_cast<const hk_f16x8*>(bu + p * (BM * 256u) + mt * 4096u);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    hk_f16x8 wh, wl;
+                    rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[mt], acc[mt][r]);
+                }
+            }
+            rows_copied();
+            __syncthreads();
+        }
+    };
+    // two supersteps a round, so the prefetched weights need no moves
+    for (uint32_t t = 0; t < n_super; t += 2u) {
+        super(t, w[0], w[1]);
+        if (t + 1u < n_super) super(t + 1u, w[1], w[0]);
+    }
+
+    int32_t exps[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) exps[mt] = sexp[16 * mt + m];
+    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
+    rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
+}
+
+template <int KIND, int WP, int XP, int MT, int FORM>
+__global__ void __launch_bounds__(256, 2) rows_tile_kernel(RowsArgs a) {
+    constexpr int BM = 16 * MT;
+    extern __shared__ __align__(16) uint8_t lds[];  // two buffers of BM x 256 XP bytes
     __shared__ uint32_t src[BM];
     __shared__ int32_t sexp[BM];
-    const int lane = threadIdx.x & 63;
-    const uint32_t wave = threadIdx.x >> 6, tid = threadIdx.x;
-
+    const uint32_t tid = threadIdx.x;
     uint32_t tile, block, group = 0, first, last;
     if constexpr (FORM == ROWS_LORA) {
         if (!rows_item(a, (a.n + BM - 1u) / BM, &tile, &block)) return;
@@ -196,102 +327,9 @@ __global__ void __launch_bounds__(256, 2) rows_tile_kernel(RowsArgs a) {
         if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
     }
     __syncthreads();
-
-    const OrganView o = a.organs[group];
-    const OrganView ou = GLU ? a.up[group] : o;
-    const uint32_t T0 = (block * 4u + wave) * (GLU ? RT / 2 : RT);
-    uint32_t T[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) T[r] = min(T0 + (uint32_t)(GLU ? r % (RT / 2) : r), a.n_row_tiles - 1u);
-    auto view = [&](int r) -> const OrganView& { return (GLU && r >= RT / 2) ? ou : o; };
-
-    // x: this thread copies chunk tid % 16 of rows tid / 16 + 16 i
-    const size_t pitch = (size_t)a.stages * 256u * XP;
-    const uint8_t* xs[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) xs[i] = a.ws.img + (size_t)src[(tid >> 4) + 16u * i] * pitch + (tid & 15u) * 16u;
-    const uint32_t xd = (tid >> 4) * 256u + (((tid & 15u) ^ (tid >> 4)) * 16u);
-    uint4 xr[MT][XP];
-    auto x_load = [&](uint32_t s) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int p = 0; p < XP; ++p) xr[i][p] = ldg(reinterpret_cast<const uint4*>(xs[i] + (size_t)s * (256u * XP) + 256u * p));
-    };
-    auto x_store = [&](uint32_t s) {
-        uint8_t* b = lds + (s & 1u) * BUF + xd;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int p = 0; p < XP; ++p) *reinterpret_cast<uint4*>(b + p * (BM * 256u) + i * 4096u) = xr[i][p];
-    };
-
-    const uint32_t n_super = a.stages / STG;
-    uint4 hdr[RT] = {};
-    auto heads = [&](uint32_t t) {
-        if constexpr (KIND == HK_MIXED) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) hdr[r] = ldg(view(r).hdr + (T[r] * view(r).steps + t));
-        }
-    };
-    RowsW<KIND> cur[RT], nxt[RT];
-    auto w_load = [&](uint32_t t, RowsW<KIND>(&w)[RT]) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) rows_fetch<KIND>(view(r), T[r], t, lane, hdr[r], w[r]);
-    };
-
-    hk_f32x4 acc[MT][RT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
-
-    x_load(0);
-    heads(0);
-    w_load(0, cur);
-    heads(min(1u, n_super - 1u));
-    x_store(0);
-    __syncthreads();
-
-    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
-    for (uint32_t t = 0; t < n_super; ++t) {
-        w_load(min(t + 1u, n_super - 1u), nxt);
-        heads(min(t + 2u, n_super - 1u));
-#pragma unroll
-        for (int st = 0; st < STG; ++st) {
-            const uint32_t s = t * STG + st;
-            x_load(min(s + 1u, a.stages - 1u));
-            const uint8_t* b = lds + (s & 1u) * BUF + m * 256u;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint8_t* bu = b + (((4u * u + q) ^ m) * 16u);
-                hk_f16x8 x[MT][XP];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int p = 0; p < XP; ++p)
-                        x[mt][p] = *reinterpret_cast<const hk_f16x8*>(bu + p * (BM * 256u) + mt * 4096u);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    hk_f16x8 wh, wl;
-                    rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[mt], acc[mt][r]);
-                }
-            }
-            // the other buffer was last read before the previous stage's barrier
-            x_store(s + 1u);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
-    }
-
-    int32_t exps[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) exps[mt] = sexp[16 * mt + m];
-    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
-    rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
+    // a tile with at most half its positions costs half the products
+    if (MT == 8 && last - first <= 64u) rows_tile<KIND, WP, XP, (MT == 8 ? 4 : MT), FORM>(a, group, first, last, block, lds, src, sexp);
+    else rows_tile<KIND, WP, XP, MT, FORM>(a, group, first, last, block, lds, src, sexp);
 }
 
 // ------------------------------------------------------------------ few rows a group: columns split over the waves
@@ -419,16 +457,16 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
 
 // ------------------------------------------------------------------ launch
 
-template <int KIND, int WP, int XP, int MT, int FORM>
+template <int KIND, int WP, int XP, int MT, int FORM, bool TILE>
 hipError_t rows_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
     constexpr uint32_t out_tiles = FORM == ROWS_GLU ? 2u : 1u;  // tiles per output tile
     const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles;
-    const uint32_t per = sh.tile ? 16u / out_tiles : 4u / sh.kw * 2u / out_tiles;
+    const uint32_t per = TILE ? 16u / out_tiles : 4u / sh.kw * 2u / out_tiles;
     a.row_blocks = (a.n_row_tiles + per - 1u) / per;
     const uint64_t items = (uint64_t)tiles * a.row_blocks, grid = (items + 7u) / 8u * 8u;
     if (grid == 0) return hipSuccess;
     if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
-    if (sh.tile) {
+    if constexpr (TILE) {
         constexpr size_t lds = 2u * 16u * MT * 256u * XP;
         auto* k = rows_tile_kernel<KIND, WP, XP, MT, FORM>;
         hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), lds, s, a);
@@ -441,12 +479,13 @@ hipError_t rows_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
 
 template <int KIND, int WP, int XP, int FORM>
 hipError_t rows_mt(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
-    switch (sh.mt) {
-    case 1: return rows_go<KIND, WP, XP, 1, FORM>(sh, a, s);
-    case 4: return rows_go<KIND, WP, XP, 4, FORM>(sh, a, s);
-    case 8:
-        if constexpr (XP == 1) return rows_go<KIND, WP, XP, 8, FORM>(sh, a, s);
-        break;
+    if (sh.tile) {
+        if (sh.mt == 4) return rows_go<KIND, WP, XP, 4, FORM, true>(sh, a, s);
+        if constexpr (XP == 1)
+            if (sh.mt == 8) return rows_go<KIND, WP, XP, 8, FORM, true>(sh, a, s);
+    } else {
+        if (sh.mt == 1) return rows_go<KIND, WP, XP, 1, FORM, false>(sh, a, s);
+        if (sh.mt == 4) return rows_go<KIND, WP, XP, 4, FORM, false>(sh, a, s);
     }
     return hipErrorInvalidValue;
 }
