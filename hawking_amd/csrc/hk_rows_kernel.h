@@ -175,12 +175,17 @@ __device__ __forceinline__ void rows_epilogue(const RowsArgs& a, uint32_t first,
 // One wave's 64 lanes copy 64 x 16 bytes from global memory to LDS at `to`
 // (wave-uniform) + 16 lane without passing through registers.  Written as
 // assembly because the compiler would make every later LDS read wait for the
-// copy; it has no outputs, and rows_copied() waits for it before the barrier
-// that publishes the buffer.
+// copy; it has no outputs, and rows_copied() waits for it (and for every load
+// issued before) ahead of the barrier that publishes the buffer.  That wait is
+// the builtin, so the compiler knows that its own loads have arrived too and
+// does not wait for them again after the next copies were issued.
 __device__ __forceinline__ void rows_copy16(const uint8_t* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
-__device__ __forceinline__ void rows_copied() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void rows_copied() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+}
 
 // A tile of 16 MT positions x this workgroup's 16 row tiles.
 //
@@ -265,24 +270,44 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
                 w_load(min(t + 1u, n_super - 1u), nxt);
                 heads(min(t + 2u, n_super - 1u));
             }
+            __builtin_amdgcn_sched_barrier(0);  // the loads stay here, a stage ahead of their use
+            // 4 MT steps of one x fragment and RT products each.  Fragments are
+            // read AHEAD steps before their products and the next product's
+            // weights are decoded among this one's: issued in blocks (all
+            // reads, all decoding, all products) the matrix cores wait for LDS
+            // and the decoder half of the time.
+            constexpr int STEPS = 4 * MT, AHEAD = XP == 2 ? 2 : 3;
             const uint8_t* b = lds + (s & 1u) * BUF + m * 256u;
+            hk_f16x8 x[AHEAD + 1][XP], wh[2][RT], wl[2][RT];
+            auto x_read = [&](int i) {
+                const uint8_t* bu = b + (((4u * (uint32_t)(i / MT) + q) ^ m) * 16u) + (i % MT) * 4096;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint8_t* bu = b + (((4u * u + q) ^ m) * 16u);
-                hk_f16x8 x[MT][XP];
+                for (int p = 0; p < XP; ++p) x[i % (AHEAD + 1)][p] = *reinterpret_cast<const hk_f16x8*>(bu + p * (BM * 256));
+            };
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+            for (int i = 0; i < AHEAD; ++i) x_read(i);
 #pragma unroll
-                    for (int p = 0; p < XP; ++p)
-                        x[mt][p] = *reinterpret_cast<const hk_f16x8*>(bu + p * (BM * 256u) + mt * 4096u);
+            for (int r = 0; r < RT; ++r) rows_weights<KIND, WP>(cur[r], st, 0, wh[0][r], wl[0][r]);
+            rows_each<STEPS>([&](auto i) {
+                constexpr int u = i / MT, mt = i % MT;
+                if constexpr (i + AHEAD < STEPS) x_read(i + AHEAD);
+                // RT weight fragments of the next product over MT steps
+                if constexpr (u < 3) {
+#pragma unroll
+                    for (int r = mt * RT / MT; r < (mt + 1) * RT / MT; ++r)
+                        rows_weights<KIND, WP>(cur[r], st, u + 1, wh[(u + 1) & 1][r], wl[(u + 1) & 1][r]);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[mt][r] = rows_mfma<WP, XP>(wh[u & 1][r], wl[u & 1][r], x[i % (AHEAD + 1)], acc[mt][r]);
+#ifdef ROWS_SCHED
+                __builtin_amdgcn_sched_group_barrier(0x100, XP, 0);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    hk_f16x8 wh, wl;
-                    rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[mt], acc[mt][r]);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, ROWS_SCHED, 0);
                 }
-            }
+#endif
+            });
             rows_copied();
             __syncthreads();
         }
