@@ -177,11 +177,11 @@ __global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __r
     }
 }
 
-// Up to GROUP_SCAN_READS id reads in all the one-launch form: measured against
-// the two-launch form at 512 and 327680 ids (see the launcher's callers' bench).
+// The one-launch form reads all ids in every workgroup, 256 threads of it.
 constexpr uint64_t GROUP_SCAN_READS = 1ull << 22;
+constexpr uint32_t GROUP_SCAN_IDS = 8192;
 
-static bool group_scans(uint32_t n, uint32_t G) { return (uint64_t)n * (G + 1u) <= GROUP_SCAN_READS; }
+static bool group_scans(uint32_t n, uint32_t G) { return n <= GROUP_SCAN_IDS && (uint64_t)n * (G + 1u) <= GROUP_SCAN_READS; }
 static uint32_t group_part_ids(uint32_t G) { return (G <= 2048u ? 16u : 4u) * GROUP_WAVE_IDS; }
 
 size_t group_rows_ws_bytes(uint32_t n, uint32_t G) {

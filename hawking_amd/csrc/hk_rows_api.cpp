@@ -28,11 +28,13 @@ int fail(hk_ctx* ctx, const char* fn, const RowsCheck& c) { return set_error(ctx
 bool exact_weights(int32_t y_type) { return y_type != HK_T_BF16; }
 int x_planes(int32_t x_type, int32_t y_type) { return x_type == HK_T_F32 && exact_weights(y_type) ? 2 : 1; }
 
+uint32_t max_tiles(uint32_t n, uint32_t groups, uint32_t tile_rows) { return n / tile_rows + std::min(groups, n); }
+
 // The launch's shape by the rows a group has on average.
-//  split  up to 16 rows a tile, the columns over the waves: bound by the
-//         weights, many small workgroups
+//  split  up to 16 rows a tile (or too few tiles to fill the device), the
+//         columns over the waves: bound by the weights, many small workgroups
 //  tile   64 or 128 rows a tile through LDS: bound by the matrix cores
-RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t n, uint32_t groups, uint32_t rows,
+RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t n, uint32_t groups, uint32_t row_tiles,
                     uint32_t stages) {
     RowsShape sh{};
     sh.kind = kind;
@@ -40,23 +42,17 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     sh.wp = exact_weights(y_type) ? 2 : 1;
     sh.xp = x_planes(x_type, y_type);
     const uint32_t per = n / std::max(1u, std::min(groups, n));
-    if (per <= 16) {
-        sh.mt = 1;
-    } else if (per <= 64 || sh.xp == 2) {
-        sh.mt = 4;
-        sh.tile = true;
-    } else {
-        sh.mt = 8;
-        sh.tile = true;
-    }
+    const bool one_plane = sh.xp == 1 && (sh.wp == 1 || kind == HK_BIN);
+    sh.mt = per <= 16 ? 1 : per <= 64 || !one_plane ? 4 : 8;
+    const uint32_t blocks = (row_tiles * (form == ROWS_GLU ? 2u : 1u) + 15u) / 16u;
+    const uint32_t tiles = std::max(std::min(groups, n), n / (16u * sh.mt));
+    sh.tile = sh.mt > 1 && (uint64_t)tiles * blocks >= 256;
+    if (!sh.tile && sh.mt > 4) sh.mt = 4;
     // columns over as many waves as have a superstep each
     const uint32_t supers = (kind == HK_BIN || kind == HK_MIXED) ? stages / 4u : stages;
     sh.kw = supers >= 4 ? 4 : supers >= 2 ? 2 : 1;
-    (void)rows;
     return sh;
 }
-
-uint32_t max_tiles(uint32_t n, uint32_t groups, uint32_t tile_rows) { return n / tile_rows + std::min(groups, n); }
 
 // Sections of a product's workspace: exps, tiles, images (and an adapter call's mid rows).
 struct WsLayout {
@@ -110,7 +106,7 @@ int grouped(hk_ctx* ctx, const char* fn, const hk_organ_set* set, const hk_organ
     if (y->n == 0) return HK_OK;
     OnDevice on(ctx);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const RowsShape sh = shape_for(f.kind, up ? ROWS_GLU : ROWS_PLAIN, x->type, y->type, y->n, set->n, f.rows, stages);
+    const RowsShape sh = shape_for(f.kind, up ? ROWS_GLU : ROWS_PLAIN, x->type, y->type, y->n, set->n, f.n_tiles, stages);
     RowsArgs a{};
     a.organs = set->dev;
     a.up = up ? up->dev : nullptr;
@@ -271,7 +267,7 @@ extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_ba
     if (y->n == 0) return HK_OK;
     OnDevice on(ctx);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const RowsShape sh = shape_for(f.kind, ROWS_LORA, x->type, y->type, y->n, 1, f.rows, stages);
+    const RowsShape sh = shape_for(f.kind, ROWS_LORA, x->type, y->type, y->n, 1, f.n_tiles, stages);
     RowsArgs a{};
     a.organs = static_cast<const OrganView*>(organ->view_dev);
     // the adapters' first half works on tiles of 16 rows of one slot

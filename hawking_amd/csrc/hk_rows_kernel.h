@@ -25,6 +25,19 @@ __device__ __forceinline__ bool rows_item(const RowsArgs& a, uint32_t n_tiles, u
     return k < per && i < items;
 }
 
+// A set's organ, read by scalar loads into scalar registers (an ordinary load
+// may not be one where the kernel also writes memory, and the view's pointers
+// would sit in vector registers that the sums need).
+__device__ __forceinline__ OrganView rows_view(const OrganView* organs, uint32_t g) {
+    typedef const __attribute__((address_space(4))) uint64_t* words;
+    static_assert(sizeof(OrganView) % 8 == 0, "whole words");
+    const words p = (words)(uintptr_t)(organs + g);
+    uint64_t v[sizeof(OrganView) / 8];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(OrganView) / 8; ++i) v[i] = p[i];
+    return __builtin_bit_cast(OrganView, v);
+}
+
 // Position p's source row in the image; an index outside the source marks the
 // row bad (its results become NaN, as a non-finite row's).
 __device__ __forceinline__ uint32_t rows_source(const RowsArgs& a, uint32_t p, bool* bad) {
@@ -225,8 +238,8 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
             for (int p = 0; p < XP; ++p) rows_copy16(b + (size_t)xo[i] * 16u + 256u * p, to + p * (BM * 256u) + i * 1024u);
     };
 
-    const OrganView o = a.organs[group];
-    const OrganView ou = GLU ? a.up[group] : o;
+    const OrganView o = rows_view(a.organs, group);
+    const OrganView ou = GLU ? rows_view(a.up, group) : o;
     const uint32_t T0 = (block * 4u + wave) * (GLU ? RT / 2 : RT);
     uint32_t T[RT];
 #pragma unroll
@@ -386,8 +399,8 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
         first = __builtin_amdgcn_readfirstlane(t.first);
         last = __builtin_amdgcn_readfirstlane(t.last);
     }
-    const OrganView o = a.organs[group];
-    const OrganView ou = GLU ? a.up[group] : o;
+    const OrganView o = rows_view(a.organs, group);
+    const OrganView ou = GLU ? rows_view(a.up, group) : o;
     const uint32_t T0 = (block * (4u / kw) + wr) * (GLU ? RT / 2 : RT);
     uint32_t T[RT];
 #pragma unroll
@@ -506,7 +519,7 @@ template <int KIND, int WP, int XP, int FORM>
 hipError_t rows_mt(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
     if (sh.tile) {
         if (sh.mt == 4) return rows_go<KIND, WP, XP, 4, FORM, true>(sh, a, s);
-        if constexpr (XP == 1)
+        if constexpr (WP == 1 && XP == 1)  // (two planes of either leave no registers for 128 rows)
             if (sh.mt == 8) return rows_go<KIND, WP, XP, 8, FORM, true>(sh, a, s);
     } else {
         if (sh.mt == 1) return rows_go<KIND, WP, XP, 1, FORM, false>(sh, a, s);
