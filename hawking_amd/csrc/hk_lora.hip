@@ -115,8 +115,8 @@ __global__ void __launch_bounds__(64 * NW) lora_shrink_kernel(RowsArgs a) {
     hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [NW - 1][RT][64]
     const int lane = threadIdx.x & 63;
     const uint32_t wave = threadIdx.x >> 6, m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
-    if (blockIdx.x >= *a.ws.n_tiles) return;
     const RowsTile tile = a.ws.tiles[blockIdx.x];
+    if (tile.first >= tile.last) return;
     const uint32_t p = min(tile.first + m, tile.last - 1u);
     const LoraSlot slot = a.lora.tab[tile.group];
     const uint32_t rt_used = min((slot.rank + 15u) / 16u, (uint32_t)RT);

@@ -216,7 +216,6 @@ struct RowsWs {
     uint8_t* img;      // [source rows][stages][planes][256 bytes]
     int32_t* exps;     // [source rows]
     RowsTile* tiles;   // [max_tiles]
-    uint32_t* n_tiles;
     uint32_t max_tiles;
 };
 
@@ -251,9 +250,9 @@ struct RowsArgs {
     void* y;
     size_t y_stride;          // elements
     int32_t y_type;
-    uint32_t y_vec;           // four rows may be stored at once
+    uint32_t y_vec;           // y's rows begin on 16 bytes
     uint32_t scatter;         // y row = order[position] (else the position)
-    uint32_t row_blocks;
+    uint32_t row_blocks, tiles;  // of the launch
     uint32_t* status;
     RowsLora lora;
 };
@@ -268,6 +267,12 @@ struct RowsShape {
     uint32_t kw;      // split kernel: waves that share a row tile's columns
 };
 constexpr int ROWS_PLAIN = 0, ROWS_GLU = 1, ROWS_LORA = 2;
+// Whether the tile kernel takes 128 positions: their sums are half of a wave's
+// registers, and two planes of either operand, an adapter's operands or the
+// wider weight fetches of q8 and mixed organs do not fit beside them.
+constexpr bool rows_tile8(int kind, int wp, int xp, int form) {
+    return wp == 1 && xp == 1 && form != ROWS_LORA && kind != HK_MIXED && kind != HK_Q8;
+}
 
 hipError_t launch_rows_image(const void* x, int x_type, size_t x_stride, uint32_t n, uint32_t cols, int kind, int planes,
                              const RowsWs& ws, const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,

@@ -75,7 +75,7 @@ __device__ void rows_tiles(const RowsWs& ws, const int32_t* offsets, uint32_t gr
         }
         base += total;
     }
-    if (tid == 0) *ws.n_tiles = min(base, ws.max_tiles);
+    for (uint32_t j = base + tid; j < ws.max_tiles; j += 256u) ws.tiles[j] = RowsTile{0u, 0u, 0u, 0u};  // no positions
 }
 
 // Rows of x -> image rows (hk_rows.h), TPR threads a row; the last block makes

@@ -42,8 +42,8 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     sh.wp = exact_weights(y_type) ? 2 : 1;
     sh.xp = x_planes(x_type, y_type);
     const uint32_t per = n / std::max(1u, std::min(groups, n));
-    const bool one_plane = sh.xp == 1 && (sh.wp == 1 || kind == HK_BIN);
-    sh.mt = per <= 16 ? 1 : per <= 64 || !one_plane ? 4 : 8;
+    const bool tile8 = rows_tile8(kind, kind == HK_BIN ? 1 : sh.wp, sh.xp, form);
+    sh.mt = per <= 16 ? 1 : per <= 64 || !tile8 ? 4 : 8;
     const uint32_t blocks = (row_tiles * (form == ROWS_GLU ? 2u : 1u) + 15u) / 16u;
     const uint32_t tiles = std::max(std::min(groups, n), n / (16u * sh.mt));
     sh.tile = sh.mt > 1 && (uint64_t)tiles * blocks >= 256;
@@ -60,7 +60,7 @@ struct WsLayout {
 };
 WsLayout ws_layout(uint32_t x_rows, uint32_t stages, int planes, uint32_t n, uint32_t groups, uint32_t kk_max, int mid_planes) {
     WsLayout L;
-    size_t at = 256;  // the tile count
+    size_t at = 0;
     L.exps = at;
     at += align256((size_t)x_rows * 4);
     L.tiles = at;
@@ -79,14 +79,14 @@ WsLayout ws_layout(uint32_t x_rows, uint32_t stages, int planes, uint32_t n, uin
 RowsWs ws_views(void* ws, const WsLayout& L, uint32_t tiles) {
     uint8_t* b = static_cast<uint8_t*>(ws);
     return {b + L.img, reinterpret_cast<int32_t*>(b + L.exps), reinterpret_cast<RowsTile*>(b + L.tiles),
-            reinterpret_cast<uint32_t*>(b), tiles};
+            tiles};
 }
 
 void set_y(RowsArgs* a, const hk_rows* y) {
     a->y = y->data;
     a->y_type = y->type;
     a->y_stride = y->stride;
-    a->y_vec = y->stride % 4 == 0 && reinterpret_cast<uintptr_t>(y->data) % (4 * type_bytes(y->type)) == 0;
+    a->y_vec = y->stride * type_bytes(y->type) % 16 == 0 && reinterpret_cast<uintptr_t>(y->data) % 16 == 0;
 }
 
 int grouped(hk_ctx* ctx, const char* fn, const hk_organ_set* set, const hk_organ_set* up, const hk_rows* x,

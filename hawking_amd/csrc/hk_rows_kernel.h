@@ -14,15 +14,37 @@
 namespace hk {
 
 // The work item of this workgroup: position tile and row block.  Workgroups
-// go to the 8 XCDs round robin; each XCD takes one contiguous run of items
-// (row blocks of a position tile, then the next tile), so the row blocks that
-// read the same x rows share its L2.
-__device__ __forceinline__ bool rows_item(const RowsArgs& a, uint32_t n_tiles, uint32_t* tile, uint32_t* block) {
-    const uint32_t items = n_tiles * a.row_blocks, per = (items + 7u) / 8u;
-    const uint32_t k = blockIdx.x >> 3, i = (blockIdx.x & 7u) * per + k;
-    *tile = i / a.row_blocks;
-    *block = i % a.row_blocks;
-    return k < per && i < items;
+// go to the 8 XCDs round robin.  With many position tiles an XCD takes every
+// eighth one with all its row blocks in a row, so the blocks that read the
+// same x rows share its L2; with few, the row blocks go round the XCDs.
+constexpr uint32_t ROWS_XCD_TILES = 32;
+__device__ __forceinline__ void rows_item(const RowsArgs& a, uint32_t* tile, uint32_t* block) {
+    if (a.tiles < ROWS_XCD_TILES) {
+        *tile = blockIdx.x / a.row_blocks;
+        *block = blockIdx.x % a.row_blocks;
+    } else {
+        const uint32_t k = blockIdx.x >> 3;
+        *tile = (k / a.row_blocks) * 8u + (blockIdx.x & 7u);
+        *block = k % a.row_blocks;
+    }
+}
+
+// This workgroup's positions; false where it has none.
+template <int FORM, int BM>
+__device__ __forceinline__ bool rows_positions(const RowsArgs& a, uint32_t tile, uint32_t* group, uint32_t* first, uint32_t* last) {
+    if constexpr (FORM == ROWS_LORA) {
+        *group = 0;
+        *first = tile * BM;
+        *last = min(*first + BM, a.n);
+        return *first < a.n;
+    } else {
+        if (tile >= a.ws.max_tiles) return false;
+        const RowsTile t = a.ws.tiles[tile];
+        *group = __builtin_amdgcn_readfirstlane(t.group);
+        *first = __builtin_amdgcn_readfirstlane(t.first);
+        *last = __builtin_amdgcn_readfirstlane(t.last);
+        return *first < *last;
+    }
 }
 
 // A set's organ, read by scalar loads into scalar registers (an ordinary load
@@ -200,6 +222,83 @@ __device__ __forceinline__ void rows_copied() {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 }
 
+// What a workgroup's waves share about its positions: the exponent of the
+// source row and the row of y.
+struct RowsMap {
+    int32_t exp;
+    uint32_t dst;
+};
+// LDS a wave has for its results on their way out: 16 positions x 64 rows of f32, padded rows.
+constexpr uint32_t ROWS_OUT_BYTES = 8192;
+
+// Scales a tile's sums back and stores them, by way of LDS: a lane holds four
+// rows of one position, so stored from the registers a position's 64 rows
+// would go out in 32-byte pieces; from LDS 16 bytes a lane make whole lines.
+// GLU: row tiles r and r + RT / 2 are the gate and the up rows of the same outputs.
+template <int MT, int RT, bool GLU>
+__device__ __forceinline__ void rows_store_tile(const RowsArgs& a, uint32_t first, uint32_t last, uint32_t T0, int lane,
+                                                const RowsMap* map, uint8_t* out, const int32_t* exps,
+                                                hk_f32x4 (&acc)[MT][RT]) {
+    constexpr int RO = GLU ? RT / 2 : RT;
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4, row0 = 16u * T0;
+    if (row0 >= a.rows) return;
+    const bool f32 = a.y_type == HK_T_F32;
+    const uint32_t es = f32 ? 4u : 2u, pitch = 16u * RO * es + 16u;
+    const uint32_t per = RO * es;                  // 16-byte pieces of a position
+    const uint32_t piece = (uint32_t)lane % per, sub = (uint32_t)lane / per, subs = 64u / per;
+    const uint32_t row = row0 + piece * 16u / es;  // this lane's first row on the way out
+    bool bad = false;
+    rows_each<MT>([&](auto mt) {
+        const uint32_t p0 = first + 16u * mt;
+        if (p0 >= last) return;  // uniform
+        const bool nan = exps[mt] == ROWS_EXP_BAD, in = p0 + m < last;
+#pragma unroll
+        for (int r = 0; r < RO; ++r) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x = nan ? __builtin_nanf("") : ldexpf(acc[mt][r][j], -exps[mt]);
+                if constexpr (GLU) x = x / (1.0f + expf(-x)) * ldexpf(acc[mt][r + RO][j], -exps[mt]);
+                bad |= in && row0 + 16u * r + 4u * q + j < a.rows && !isfinite(x);
+                v[j] = x;
+            }
+            uint8_t* at = out + m * pitch + (16u * r + 4u * q) * es;
+            if (f32) {
+                *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = a.y_type == HK_T_BF16 ? f32_to_bf16_bits(v[j]) : f32_to_f16_bits(v[j]);
+                *reinterpret_cast<uint2*>(at) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+            }
+        }
+        wave_lds_sync();
+        for (uint32_t s = sub; s < 16u; s += subs) {
+            if (p0 + s >= last) break;
+            const uint32_t dst = map[16u * mt + s].dst;
+            if (dst >= a.n) continue;  // a scattered row outside y (flagged when the map was made)
+            const uint4 v = *reinterpret_cast<const uint4*>(out + s * pitch + piece * 16u);
+            uint8_t* to = static_cast<uint8_t*>(a.y) + ((size_t)dst * a.y_stride + row) * es;
+            if (a.y_vec && row + 16u / es <= a.rows) {
+                *reinterpret_cast<uint4*>(to) = v;
+            } else {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    if (f32) {
+                        if (row + k < a.rows) reinterpret_cast<uint32_t*>(to)[k] = w[k];
+                    } else {
+                        if (row + 2u * k < a.rows) reinterpret_cast<uint16_t*>(to)[2 * k] = (uint16_t)w[k];
+                        if (row + 2u * k + 1u < a.rows) reinterpret_cast<uint16_t*>(to)[2 * k + 1] = (uint16_t)(w[k] >> 16);
+                    }
+                }
+            }
+        }
+        wave_lds_sync();
+    });
+    if (__ballot(bad) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
+}
+
 // A tile of 16 MT positions x this workgroup's 16 row tiles.
 //
 // Four waves, four row tiles each (SwiGLU: two gate and two up).  Per stage
@@ -211,7 +310,7 @@ __device__ __forceinline__ void rows_copied() {
 // touches lie in 16 different bank groups.
 template <int KIND, int WP, int XP, int MT, int FORM>
 __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uint32_t first, uint32_t last, uint32_t block,
-                                          uint8_t* lds, const uint32_t* src, const int32_t* sexp) {
+                                          uint8_t* lds, RowsMap* map) {
     constexpr int RT = 4, BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
     constexpr bool GLU = FORM == ROWS_GLU;
     constexpr uint32_t BUF = BM * 256u * XP;
@@ -223,11 +322,11 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
     // fills place l % 16 of its row
     const size_t pitch16 = (size_t)a.stages * 16u * XP;  // image pitch in 16-byte chunks
     uint32_t xo[MT];
+    bool no[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const uint32_t row = wave * (4u * MT) + 4u * i + q;
-        xo[i] = (uint32_t)(src[row] * pitch16) + (m ^ (row & 15u));
-    }
+    for (int i = 0; i < MT; ++i) xo[i] = rows_source(a, min(first + wave * (4u * MT) + 4u * i + q, last - 1u), &no[i]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xo[i] = (uint32_t)(xo[i] * pitch16) + (m ^ ((wave * (4u * MT) + 4u * i + q) & 15u));
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * (4u * MT) * 256u;
     auto x_copy = [&](uint32_t s) {
         const uint8_t* b = a.ws.img + (size_t)s * (256u * XP);
@@ -266,10 +365,18 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
 
-    x_copy(0);
     heads(0);
     w_load(0, w[0]);
     heads(min(1u, n_super - 1u));
+    x_copy(0);
+    if (threadIdx.x < (uint32_t)BM) {
+        // (after the loads above, so that they do not wait for this chain)
+        const uint32_t p = min(first + threadIdx.x, last - 1u);
+        bool bad;
+        const uint32_t r = rows_source(a, p, &bad);
+        map[threadIdx.x] = {bad ? ROWS_EXP_BAD : a.ws.exps[r], a.scatter && a.order ? (uint32_t)a.order[p] : p};
+        if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
+    }
     rows_copied();
     __syncthreads();
 
@@ -333,41 +440,31 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
 
     int32_t exps[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) exps[mt] = sexp[16 * mt + m];
+    for (int mt = 0; mt < MT; ++mt) exps[mt] = map[16 * mt + m].exp;
     if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
-    rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
+    // (the last stage ended with a barrier: its buffers are free)
+    rows_store_tile<MT, RT, GLU>(a, first, last, T0, lane, map, lds + wave * ROWS_OUT_BYTES, exps, acc);
 }
 
 template <int KIND, int WP, int XP, int MT, int FORM>
-__global__ void __launch_bounds__(256, 2) rows_tile_kernel(RowsArgs a) {
+__global__ void __launch_bounds__(256, MT == 4 && WP == 1 && XP == 1 && KIND != HK_MIXED && KIND != HK_Q8 ? 3 : 2) rows_tile_kernel(RowsArgs a) {
     constexpr int BM = 16 * MT;
     extern __shared__ __align__(16) uint8_t lds[];  // two buffers of BM x 256 XP bytes
-    __shared__ uint32_t src[BM];
-    __shared__ int32_t sexp[BM];
-    const uint32_t tid = threadIdx.x;
-    uint32_t tile, block, group = 0, first, last;
-    if constexpr (FORM == ROWS_LORA) {
-        if (!rows_item(a, (a.n + BM - 1u) / BM, &tile, &block)) return;
-        first = tile * BM;
-        last = min(first + BM, a.n);
+    __shared__ RowsMap map[BM];
+    uint32_t tile, block, group, first, last;
+    rows_item(a, &tile, &block);
+    if (!rows_positions<FORM, BM>(a, tile, &group, &first, &last)) return;
+    // a tile that is not full costs its 32s of positions
+    const uint32_t mts = (last - first + 15u) / 16u;
+    if constexpr (MT == 8) {
+        if (mts > 6u) rows_tile<KIND, WP, XP, 8, FORM>(a, group, first, last, block, lds, map);
+        else if (mts > 4u) rows_tile<KIND, WP, XP, 6, FORM>(a, group, first, last, block, lds, map);
+        else if (mts > 2u) rows_tile<KIND, WP, XP, 4, FORM>(a, group, first, last, block, lds, map);
+        else rows_tile<KIND, WP, XP, 2, FORM>(a, group, first, last, block, lds, map);
     } else {
-        if (!rows_item(a, *a.ws.n_tiles, &tile, &block)) return;
-        const RowsTile t = a.ws.tiles[tile];
-        group = __builtin_amdgcn_readfirstlane(t.group);
-        first = __builtin_amdgcn_readfirstlane(t.first);
-        last = __builtin_amdgcn_readfirstlane(t.last);
+        if (mts > 2u) rows_tile<KIND, WP, XP, 4, FORM>(a, group, first, last, block, lds, map);
+        else rows_tile<KIND, WP, XP, 2, FORM>(a, group, first, last, block, lds, map);
     }
-    if (tid < (uint32_t)BM) {
-        bool bad = false;
-        const uint32_t p = min(first + tid, last - 1u), r = rows_source(a, p, &bad);
-        src[tid] = r;
-        sexp[tid] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
-        if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
-    }
-    __syncthreads();
-    // a tile with at most half its positions costs half the products
-    if (MT == 8 && last - first <= 64u) rows_tile<KIND, WP, XP, (MT == 8 ? 4 : MT), FORM>(a, group, first, last, block, lds, src, sexp);
-    else rows_tile<KIND, WP, XP, MT, FORM>(a, group, first, last, block, lds, src, sexp);
 }
 
 // ------------------------------------------------------------------ few rows a group: columns split over the waves
@@ -387,18 +484,9 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
     const uint32_t wave = threadIdx.x >> 6, wk = wave % kw, wr = wave / kw;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
 
-    uint32_t tile, block, group = 0, first, last;
-    if constexpr (FORM == ROWS_LORA) {
-        if (!rows_item(a, (a.n + BM - 1u) / BM, &tile, &block)) return;
-        first = tile * BM;
-        last = min(first + BM, a.n);
-    } else {
-        if (!rows_item(a, *a.ws.n_tiles, &tile, &block)) return;
-        const RowsTile t = a.ws.tiles[tile];
-        group = __builtin_amdgcn_readfirstlane(t.group);
-        first = __builtin_amdgcn_readfirstlane(t.first);
-        last = __builtin_amdgcn_readfirstlane(t.last);
-    }
+    uint32_t tile, block, group, first, last;
+    rows_item(a, &tile, &block);
+    if (!rows_positions<FORM, BM>(a, tile, &group, &first, &last)) return;
     const OrganView o = rows_view(a.organs, group);
     const OrganView ou = GLU ? rows_view(a.up, group) : o;
     const uint32_t T0 = (block * (4u / kw) + wr) * (GLU ? RT / 2 : RT);
@@ -501,7 +589,8 @@ hipError_t rows_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
     const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles;
     const uint32_t per = TILE ? 16u / out_tiles : 4u / sh.kw * 2u / out_tiles;
     a.row_blocks = (a.n_row_tiles + per - 1u) / per;
-    const uint64_t items = (uint64_t)tiles * a.row_blocks, grid = (items + 7u) / 8u * 8u;
+    a.tiles = tiles;
+    const uint64_t grid = (tiles < ROWS_XCD_TILES ? (uint64_t)tiles : ((uint64_t)tiles + 7u) / 8u * 8u) * a.row_blocks;
     if (grid == 0) return hipSuccess;
     if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
     if constexpr (TILE) {
@@ -519,7 +608,7 @@ template <int KIND, int WP, int XP, int FORM>
 hipError_t rows_mt(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
     if (sh.tile) {
         if (sh.mt == 4) return rows_go<KIND, WP, XP, 4, FORM, true>(sh, a, s);
-        if constexpr (WP == 1 && XP == 1)  // (two planes of either leave no registers for 128 rows)
+        if constexpr (rows_tile8(KIND, WP, XP, FORM))
             if (sh.mt == 8) return rows_go<KIND, WP, XP, 8, FORM, true>(sh, a, s);
     } else {
         if (sh.mt == 1) return rows_go<KIND, WP, XP, 1, FORM, false>(sh, a, s);
