@@ -281,11 +281,16 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// f32 -> bf16 bits, round to nearest even; a NaN stays one.
-__device__ __forceinline__ uint16_t f32_to_bf16_bits(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((b >> 16) | 0x40u);
-    return (uint16_t)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
+// f32 -> bf16 or f16 bits, round to nearest even; a NaN stays one.  (gfx950
+// converts a pair to bf16 in one instruction.)
+typedef __bf16 hk_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float hk_f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f32x2_to_bf16_bits(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(hk_f32x2{lo, hi}, hk_bf16x2));
+}
+__device__ __forceinline__ uint16_t f32_to_bf16_bits(float v) { return (uint16_t)f32x2_to_bf16_bits(v, 0.0f); }
+__device__ __forceinline__ uint32_t f32x2_to_f16_bits(float lo, float hi) {
+    return (uint32_t)f32_to_f16_bits(lo) | ((uint32_t)f32_to_f16_bits(hi) << 16);
 }
 
 // ------------------------------------------------------------------ host error plumbing

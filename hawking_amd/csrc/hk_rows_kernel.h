@@ -69,6 +69,39 @@ __device__ __forceinline__ uint32_t rows_source(const RowsArgs& a, uint32_t p, b
     return *bad ? 0u : r;
 }
 
+__device__ __forceinline__ uint2 rows_half4(int32_t type, const float (&v)[4]) {
+    if (type == HK_T_BF16) return make_uint2(f32x2_to_bf16_bits(v[0], v[1]), f32x2_to_bf16_bits(v[2], v[3]));
+    return make_uint2(f32x2_to_f16_bits(v[0], v[1]), f32x2_to_f16_bits(v[2], v[3]));
+}
+
+// silu(v) = v / (1 + e^-v) on the hardware's exp2 and reciprocal (each within
+// one step): e^-v = 2^t 2^r with t = -v log2 e rounded and r what the rounding
+// and log2 e's own lost, 2^r = 1 + r ln 2 to f32.  About 3 steps of the result;
+// expf and an exact division cost three times the instructions.
+__device__ __forceinline__ float rows_silu(float v) {
+    constexpr float L = 0x1.715476p+0f, L_LO = 0x1.4ae0bep-26f;  // log2 e = L + L_LO
+    const float t = -v * L;
+    const float r = __builtin_fmaf(-v, L, -t) - v * L_LO;
+    const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, 0x1.62e430p-1f, 1.0f);
+    return v * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// A lane's sums of one position scaled back: v[j] = acc[j] 2^-e, NaN for a bad
+// row; *fin becomes NaN if a result is not finite.
+template <bool GLU>
+__device__ __forceinline__ void rows_scale(const hk_f32x4& g, const hk_f32x4& u, int32_t e, float (&v)[4], float* fin) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = ldexpf(g[j], -e);
+        if constexpr (GLU) v[j] = rows_silu(v[j]) * ldexpf(u[j], -e);
+    }
+    if (__ballot(e == ROWS_EXP_BAD)) {
+        if (e == ROWS_EXP_BAD) v[0] = v[1] = v[2] = v[3] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *fin = __builtin_fmaf(v[j], 0.0f, *fin);
+}
+
 // Rows row .. row + 3 of y's row `yr`.
 __device__ __forceinline__ void rows_store(const RowsArgs& a, uint32_t yr, uint32_t row, const float (&v)[4]) {
     const size_t at = (size_t)yr * a.y_stride + row;
@@ -76,10 +109,7 @@ __device__ __forceinline__ void rows_store(const RowsArgs& a, uint32_t yr, uint3
         if (a.y_type == HK_T_F32) {
             *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-            uint32_t h[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = a.y_type == HK_T_BF16 ? f32_to_bf16_bits(v[i]) : f32_to_f16_bits(v[i]);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = rows_half4(a.y_type, v);
         }
         return;
     }
@@ -175,34 +205,22 @@ __device__ __forceinline__ void rows_epilogue(const RowsArgs& a, uint32_t first,
                                               const int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
     constexpr int RO = GLU ? RT / 2 : RT;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
-    bool bad = false;
+    float fin = 0.0f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const uint32_t p = first + 16u * mt + m;
-        if (p >= last) continue;
         uint32_t yr = p;
-        if (a.scatter && a.order) yr = (uint32_t)a.order[p];
-        if (yr >= a.n) continue;  // flagged by the staging
-        const bool nan = exps[mt] == ROWS_EXP_BAD;
+        if (a.scatter && a.order && p < last) yr = (uint32_t)a.order[p];
 #pragma unroll
         for (int r = 0; r < RO; ++r) {
             const uint32_t row = 16u * (T0 + (uint32_t)r) + 4u * q;
-            if (row >= a.rows) continue;
             float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float x = nan ? __builtin_nanf("") : ldexpf(acc[mt][r][j], -exps[mt]);
-                if constexpr (GLU) {
-                    const float up = ldexpf(acc[mt][r + RO][j], -exps[mt]);
-                    x = x / (1.0f + expf(-x)) * up;
-                }
-                bad |= !isfinite(x);
-                v[j] = x;
-            }
-            rows_store(a, yr, row, v);
+            rows_scale<GLU>(acc[mt][r], acc[mt][GLU ? r + RO : r], exps[mt], v, &fin);
+            // (a scattered row outside y was flagged when its source was looked up)
+            if (p < last && yr < a.n && row < a.rows) rows_store(a, yr, row, v);
         }
     }
-    if (__ballot(bad) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
+    if (__ballot(fin != fin) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
 }
 
 // ------------------------------------------------------------------ many rows a group: x through LDS
@@ -247,30 +265,17 @@ __device__ __forceinline__ void rows_store_tile(const RowsArgs& a, uint32_t firs
     const uint32_t per = RO * es;                  // 16-byte pieces of a position
     const uint32_t piece = (uint32_t)lane % per, sub = (uint32_t)lane / per, subs = 64u / per;
     const uint32_t row = row0 + piece * 16u / es;  // this lane's first row on the way out
-    bool bad = false;
+    float fin = 0.0f;
     rows_each<MT>([&](auto mt) {
         const uint32_t p0 = first + 16u * mt;
         if (p0 >= last) return;  // uniform
-        const bool nan = exps[mt] == ROWS_EXP_BAD, in = p0 + m < last;
 #pragma unroll
         for (int r = 0; r < RO; ++r) {
             float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float x = nan ? __builtin_nanf("") : ldexpf(acc[mt][r][j], -exps[mt]);
-                if constexpr (GLU) x = x / (1.0f + expf(-x)) * ldexpf(acc[mt][r + RO][j], -exps[mt]);
-                bad |= in && row0 + 16u * r + 4u * q + j < a.rows && !isfinite(x);
-                v[j] = x;
-            }
+            rows_scale<GLU>(acc[mt][r], acc[mt][GLU ? r + RO : r], exps[mt], v, &fin);
             uint8_t* at = out + m * pitch + (16u * r + 4u * q) * es;
-            if (f32) {
-                *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-                uint32_t h[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = a.y_type == HK_T_BF16 ? f32_to_bf16_bits(v[j]) : f32_to_f16_bits(v[j]);
-                *reinterpret_cast<uint2*>(at) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-            }
+            if (f32) *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2*>(at) = rows_half4(a.y_type, v);
         }
         wave_lds_sync();
         for (uint32_t s = sub; s < 16u; s += subs) {
@@ -296,7 +301,7 @@ __device__ __forceinline__ void rows_store_tile(const RowsArgs& a, uint32_t firs
         }
         wave_lds_sync();
     });
-    if (__ballot(bad) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
+    if (__ballot(fin != fin) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
 }
 
 // A tile of 16 MT positions x this workgroup's 16 row tiles.
