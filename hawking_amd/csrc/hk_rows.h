@@ -246,7 +246,7 @@ struct RowsArgs {
     const int32_t* order;     // position -> flat index, or null
     uint32_t per_row;         // flat indexes of a source row
     uint32_t n, n_src;        // positions, source rows
-    uint32_t groups, rows, n_row_tiles, stages;
+    uint32_t groups, rows, cols, n_row_tiles, stages;
     void* y;
     size_t y_stride;          // elements
     int32_t y_type;
@@ -265,6 +265,8 @@ struct RowsShape {
     int mt;           // 16-row tiles of positions
     bool tile;        // the tile kernel (x in LDS), else the split kernel
     uint32_t kw;      // split kernel: waves that share a row tile's columns
+    bool vec;         // the int8 engine: tile_rows positions a tile, block_tiles row tiles a workgroup
+    uint32_t tile_rows, block_tiles;
 };
 constexpr int ROWS_PLAIN = 0, ROWS_GLU = 1, ROWS_LORA = 2;
 // Whether the tile kernel takes 128 positions: their sums are half of a wave's
@@ -290,7 +292,27 @@ hipError_t launch_combine_rows(const void* x, int x_type, size_t xs, uint32_t n,
                                uint32_t tokens, uint32_t per_row, uint32_t cols, const void* base, int base_type, size_t bs,
                                void* y, int y_type, size_t ys, hipStream_t s);
 hipError_t launch_rows_product(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
+// Bytes of a row's int8 image, and the images (and tiles) of a product that uses them.
+size_t rows_vec_image_bytes(int kind, uint32_t cols);
+hipError_t launch_rows_vec_image(const void* x, int x_type, size_t x_stride, uint32_t n, uint32_t cols, int kind,
+                                 const RowsWs& ws, const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                 uint32_t* status, hipStream_t s);
 // one translation unit a kind
+hipError_t launch_rows_vec_image_q4(const void* x, int type, size_t stride, uint32_t n, uint32_t cols, const RowsWs& ws,
+                                     const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                     uint32_t* status, hipStream_t s);
+hipError_t launch_rows_vec_image_q8(const void* x, int type, size_t stride, uint32_t n, uint32_t cols, const RowsWs& ws,
+                                     const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                     uint32_t* status, hipStream_t s);
+hipError_t launch_rows_vec_image_u3(const void* x, int type, size_t stride, uint32_t n, uint32_t cols, const RowsWs& ws,
+                                     const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                     uint32_t* status, hipStream_t s);
+hipError_t launch_rows_vec_image_bin(const void* x, int type, size_t stride, uint32_t n, uint32_t cols, const RowsWs& ws,
+                                     const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                     uint32_t* status, hipStream_t s);
+hipError_t launch_rows_vec_image_mixed(const void* x, int type, size_t stride, uint32_t n, uint32_t cols, const RowsWs& ws,
+                                     const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                     uint32_t* status, hipStream_t s);
 hipError_t launch_rows_q4(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
 hipError_t launch_rows_q8(const RowsShape& sh, const RowsArgs& a, hipStream_t s);
 hipError_t launch_rows_u3(const RowsShape& sh, const RowsArgs& a, hipStream_t s);

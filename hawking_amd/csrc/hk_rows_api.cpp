@@ -30,17 +30,41 @@ int x_planes(int32_t x_type, int32_t y_type) { return x_type == HK_T_F32 && exac
 
 uint32_t max_tiles(uint32_t n, uint32_t groups, uint32_t tile_rows) { return n / tile_rows + std::min(groups, n); }
 
+// Rows a group, on average, up to which a product takes the int8 engine, and
+// the LDS its images may have (two workgroups a CU).
+constexpr uint32_t VEC_ROWS = 4;
+constexpr size_t VEC_LDS = 64 * 1024;
+
+// The int8 engine wants few rows a group.  (The bound on the source rows makes
+// the workspace of a larger batch enough for every smaller one.)
+bool takes_vec(int kind, int form, uint32_t n, uint32_t groups, uint32_t x_rows, uint32_t cols) {
+    return form != ROWS_LORA && n / std::max(1u, std::min(groups, n)) <= VEC_ROWS && x_rows <= (VEC_ROWS + 1u) * groups &&
+           rows_vec_image_bytes(kind, cols) <= VEC_LDS;
+}
+
 // The launch's shape by the rows a group has on average.
+//  vec    up to 4: the int8 engine, bound by the weight stream
 //  split  up to 16 rows a tile (or too few tiles to fill the device), the
-//         columns over the waves: bound by the weights, many small workgroups
+//         columns over the waves
 //  tile   64 or 128 rows a tile through LDS: bound by the matrix cores
-RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t n, uint32_t groups, uint32_t row_tiles,
-                    uint32_t stages) {
+RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t n, uint32_t groups, uint32_t x_rows,
+                    uint32_t cols, uint32_t row_tiles) {
     RowsShape sh{};
     sh.kind = kind;
     sh.form = form;
     sh.wp = exact_weights(y_type) ? 2 : 1;
     sh.xp = x_planes(x_type, y_type);
+    if (takes_vec(kind, form, n, groups, x_rows, cols)) {
+        sh.vec = true;
+        const size_t img = rows_vec_image_bytes(kind, cols);
+        sh.tile_rows = img * 4 <= VEC_LDS ? 4 : img * 2 <= VEC_LDS ? 2 : 1;
+        // a workgroup's row tiles: whole rounds of its waves, and about 2048 workgroups in all
+        const uint32_t round = form == ROWS_GLU ? 4 : 8, tiles = std::min(groups, n);
+        const uint32_t most = (uint32_t)(((uint64_t)row_tiles * tiles + 2047u) / 2048u);
+        sh.block_tiles = std::max(1u, (most + round - 1u) / round) * round;
+        return sh;
+    }
+    const uint32_t stages = rows_stages(kind, cols);
     const uint32_t per = n / std::max(1u, std::min(groups, n));
     const bool tile8 = rows_tile8(kind, kind == HK_BIN ? 1 : sh.wp, sh.xp, form);
     sh.mt = per <= 16 ? 1 : per <= 64 || !tile8 ? 4 : 8;
@@ -48,6 +72,7 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     const uint32_t tiles = std::max(std::min(groups, n), n / (16u * sh.mt));
     sh.tile = sh.mt > 1 && (uint64_t)tiles * blocks >= 256;
     if (!sh.tile && sh.mt > 4) sh.mt = 4;
+    sh.tile_rows = 16u * sh.mt;
     // columns over as many waves as have a superstep each
     const uint32_t supers = (kind == HK_BIN || kind == HK_MIXED) ? stages / 4u : stages;
     sh.kw = supers >= 4 ? 4 : supers >= 2 ? 2 : 1;
@@ -58,13 +83,17 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
 struct WsLayout {
     size_t exps = 0, tiles = 0, mid_exps = 0, mid = 0, img = 0, total = 0;
 };
-WsLayout ws_layout(uint32_t x_rows, uint32_t stages, int planes, uint32_t n, uint32_t groups, uint32_t kk_max, int mid_planes) {
+WsLayout ws_layout(int kind, uint32_t cols, uint32_t x_rows, int planes, uint32_t n, uint32_t groups, uint32_t kk_max,
+                   int mid_planes) {
     WsLayout L;
+    // enough for every batch up to this one: smaller ones may take the int8 engine
+    const uint32_t vec_n = kk_max ? 0 : std::min(n, (VEC_ROWS + 1u) * groups);
+    const uint32_t vec_x = kk_max || rows_vec_image_bytes(kind, cols) > VEC_LDS ? 0 : std::min(x_rows, (VEC_ROWS + 1u) * groups);
     size_t at = 0;
     L.exps = at;
     at += align256((size_t)x_rows * 4);
     L.tiles = at;
-    at += align256((size_t)max_tiles(n, groups, 16) * sizeof(RowsTile));
+    at += align256((size_t)std::max(max_tiles(n, groups, 16), max_tiles(vec_n, groups, 1)) * sizeof(RowsTile));
     if (kk_max) {
         L.mid_exps = at;
         at += align256((size_t)n * 4);
@@ -72,7 +101,7 @@ WsLayout ws_layout(uint32_t x_rows, uint32_t stages, int planes, uint32_t n, uin
         at += align256((size_t)n * kk_max * 64u * mid_planes);
     }
     L.img = at;
-    L.total = at + (size_t)x_rows * stages * 256u * planes;
+    L.total = at + std::max((size_t)x_rows * rows_stages(kind, cols) * 256u * planes, (size_t)vec_x * rows_vec_image_bytes(kind, cols));
     return L;
 }
 
@@ -99,18 +128,17 @@ int grouped(hk_ctx* ctx, const char* fn, const hk_organ_set* set, const hk_organ
                up->first.group != f.group))
         return set_error(ctx, HK_E_GEOMETRY, std::string(fn) + ": the gate and up sets must share kind, shape and size");
     const int kind = set->res_dev || (up && up->res_dev) ? HK_BIN_RICE : f.kind;
-    const uint32_t stages = rows_stages(f.kind, f.cols);
-    const WsLayout L = x && y ? ws_layout(x->n, stages, x_planes(x->type, y->type), y->n, set->n, 0, 0) : WsLayout{};
+    const WsLayout L = x && y ? ws_layout(f.kind, f.cols, x->n, x_planes(x->type, y->type), y->n, set->n, 0, 0) : WsLayout{};
     const RowsCheck c = check_product(kind, f.rows, f.cols, x, order, per_row, offsets, y, ws, ws_bytes, L.total);
     if (!c.ok()) return fail(ctx, fn, c);
     if (y->n == 0) return HK_OK;
     OnDevice on(ctx);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const RowsShape sh = shape_for(f.kind, up ? ROWS_GLU : ROWS_PLAIN, x->type, y->type, y->n, set->n, f.n_tiles, stages);
+    const RowsShape sh = shape_for(f.kind, up ? ROWS_GLU : ROWS_PLAIN, x->type, y->type, y->n, set->n, x->n, f.cols, f.n_tiles);
     RowsArgs a{};
     a.organs = set->dev;
     a.up = up ? up->dev : nullptr;
-    a.ws = ws_views(ws, L, max_tiles(y->n, set->n, 16u * sh.mt));
+    a.ws = ws_views(ws, L, max_tiles(y->n, set->n, sh.tile_rows));
     a.order = order;
     a.per_row = order ? per_row : 1u;
     a.n = y->n;
@@ -118,11 +146,14 @@ int grouped(hk_ctx* ctx, const char* fn, const hk_organ_set* set, const hk_organ
     a.groups = set->n;
     a.rows = f.rows;
     a.n_row_tiles = f.n_tiles;
-    a.stages = stages;
+    a.cols = f.cols;
+    a.stages = rows_stages(f.kind, f.cols);
     a.status = ctx->dev_status;
     set_y(&a, y);
-    int rc = check_hip(ctx, launch_rows_image(x->data, x->type, x->stride, x->n, f.cols, f.kind, sh.xp, a.ws, offsets, set->n,
-                                              y->n, 16u * sh.mt, ctx->dev_status, st),
+    int rc = check_hip(ctx, sh.vec ? launch_rows_vec_image(x->data, x->type, x->stride, x->n, f.cols, f.kind, a.ws, offsets, set->n,
+                                                           y->n, sh.tile_rows, ctx->dev_status, st)
+                                   : launch_rows_image(x->data, x->type, x->stride, x->n, f.cols, f.kind, sh.xp, a.ws, offsets,
+                                                       set->n, y->n, sh.tile_rows, ctx->dev_status, st),
                        "row image launch");
     if (!rc) rc = check_hip(ctx, launch_rows_product(sh, a, st), "row product launch");
     return rc;
@@ -155,7 +186,7 @@ extern "C" int hk_group_rows(hk_ctx* ctx, const int32_t* ids, uint32_t n, uint32
 extern "C" size_t hk_gemm_grouped_workspace(const hk_organ_set* set, uint32_t x_rows, int32_t x_type, uint32_t n,
                                             int32_t y_type) {
     if (!set) return 0;
-    return ws_layout(x_rows, rows_stages(set->first.kind, set->first.cols), x_planes(x_type, y_type), n, set->n, 0, 0).total;
+    return ws_layout(set->first.kind, set->first.cols, x_rows, x_planes(x_type, y_type), n, set->n, 0, 0).total;
 }
 
 extern "C" int hk_gemm_grouped(hk_ctx* ctx, const hk_organ_set* set, const hk_rows* x, const int32_t* order, uint32_t per_row,
@@ -243,7 +274,7 @@ extern "C" int hk_lora_bank_set(hk_ctx* ctx, hk_lora_bank* bank, uint32_t slot, 
 
 extern "C" size_t hk_gemm_lora_workspace(const hk_lora_bank* bank, uint32_t n, int32_t x_type, int32_t y_type) {
     if (!bank) return 0;
-    return ws_layout(n, rows_stages(bank->kind, bank->cols), x_planes(x_type, y_type), n, bank->n_slots, bank->kk_max,
+    return ws_layout(bank->kind, bank->cols, n, x_planes(x_type, y_type), n, bank->n_slots, bank->kk_max,
                      exact_weights(y_type) ? 2 : 1).total;
 }
 
@@ -259,7 +290,7 @@ extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_ba
     if (x && y && x->n != y->n) return set_error(ctx, HK_E_GEOMETRY, "hk_gemm_lora: x and y need as many rows");
     const uint32_t stages = rows_stages(f.kind, f.cols);
     const int mid_planes = y && exact_weights(y->type) ? 2 : 1;
-    const WsLayout L = x && y ? ws_layout(x->n, stages, x_planes(x->type, y->type), y->n, bank->n_slots, bank->kk_max, mid_planes)
+    const WsLayout L = x && y ? ws_layout(f.kind, f.cols, x->n, x_planes(x->type, y->type), y->n, bank->n_slots, bank->kk_max, mid_planes)
                               : WsLayout{};
     const RowsCheck c = check_product(organ->res_dev ? HK_BIN_RICE : f.kind, f.rows, f.cols, x, order, 1, offsets, y, ws, ws_bytes,
                                       L.total);
@@ -267,7 +298,7 @@ extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_ba
     if (y->n == 0) return HK_OK;
     OnDevice on(ctx);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const RowsShape sh = shape_for(f.kind, ROWS_LORA, x->type, y->type, y->n, 1, f.n_tiles, stages);
+    const RowsShape sh = shape_for(f.kind, ROWS_LORA, x->type, y->type, y->n, 1, x->n, f.cols, f.n_tiles);
     RowsArgs a{};
     a.organs = static_cast<const OrganView*>(organ->view_dev);
     // the adapters' first half works on tiles of 16 rows of one slot
@@ -279,6 +310,7 @@ extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_ba
     a.groups = 1;
     a.rows = f.rows;
     a.n_row_tiles = f.n_tiles;
+    a.cols = f.cols;
     a.stages = stages;
     a.scatter = 1;
     a.status = ctx->dev_status;

@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "hk_rows.h"
+#include "hk_rows_image.h"
 
 namespace hk {
 
@@ -586,6 +587,219 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
     rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
 }
 
+// ------------------------------------------------------------------ one to four rows a group: the GEMV engine
+
+// With so few rows a group the weight stream is the bound, and decoding to f16
+// alone (1.6 instructions a weight) takes longer than HBM needs for it.  The
+// int8 engine of hk_mfma.h decodes a quarter of that a weight, and its x image
+// (24-bit fixed point a unit) gives f32 accuracy, so these calls use it: a
+// workgroup keeps the images of up to 4 positions of one group in LDS and each
+// of its waves streams RT = 2 row tiles at a time (SwiGLU: one of the gate, one
+// of the up organ) past all of them, the tiles' steps in one run with DEPTH
+// steps of loads in flight.
+
+// Rows of x -> int8 images (a row a workgroup, 2048 columns at a time through
+// LDS); the last block makes the product's tiles.
+template <int KIND>
+__global__ void __launch_bounds__(256) rows_vec_image_kernel(const void* x, int type, size_t stride, uint32_t n, uint32_t cols,
+                                                             bool vec, RowsWs ws, const int32_t* offsets, uint32_t groups,
+                                                             uint32_t n_pos, uint32_t tile_rows, uint32_t* status) {
+    constexpr uint32_t SC = Kcfg<KIND>::STEP_COLS, UNIT_FLOATS = Kcfg<KIND>::SXW, PART = 2048;
+    __shared__ __align__(16) float xs[PART];
+    __shared__ uint32_t pre[256];
+    __shared__ uint32_t bad_s;
+    if (blockIdx.x == gridDim.x - 1u) {
+        rows_tiles(ws, offsets, groups, n_pos, tile_rows, pre);
+        return;
+    }
+    const uint32_t row = blockIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t steps = (cols + SC - 1u) / SC, icols = steps * SC;
+    uint8_t* img = ws.img + (size_t)row * x_lds_bytes<KIND>(steps);
+    float* sx = reinterpret_cast<float*>(img + (size_t)steps * Kcfg<KIND>::P * A_TILE_STRIDE);
+    if (threadIdx.x == 0) bad_s = 0;
+    for (uint32_t c0 = 0; c0 < icols; c0 += PART) {
+        __syncthreads();
+        float v[8];
+        const uint32_t c = c0 + 8u * threadIdx.x;
+        if (c < cols) {  // columns come in whole 32s
+            row_load4(type, x, (size_t)row * stride + c, vec, v);
+            row_load4(type, x, (size_t)row * stride + c + 4, vec, v + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+        float4* o = reinterpret_cast<float4*>(xs + 8u * threadIdx.x);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+        __syncthreads();
+        // this wave's 512 columns are whole steps
+        const uint32_t b = c0 + 512u * wave, e = min(b + 512u, icols);
+        if (b < e) {
+            bool nf = false;
+            image_wave<KIND>(lane, xs - c0, cols, img + (size_t)(b / SC) * Kcfg<KIND>::P * A_TILE_STRIDE,
+                             sx + (size_t)(b / Kcfg<KIND>::SXG) * UNIT_FLOATS, b / 8u, e / 8u, &nf);
+            if (__ballot(nf) && lane == 0) bad_s = 1;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        ws.exps[row] = bad_s ? ROWS_EXP_BAD : 0;
+        if (bad_s) atomicOr(status, ROWS_ERR_NONFINITE);
+    }
+}
+
+// NP positions (images at lds + p bytes) x this wave's row tile pairs.
+template <int KIND, int NP, int FORM>
+__device__ __forceinline__ void rows_vec(const RowsArgs& a, const OrganView& o, const OrganView& ou, uint32_t first,
+                                         uint32_t last, uint32_t t_begin, uint32_t t_end, uint32_t wave, const uint8_t* lds,
+                                         uint32_t img_bytes, const int32_t* exps) {
+    constexpr bool GLU = FORM == ROWS_GLU;
+    constexpr int DEPTH = 3;
+    constexpr uint32_t PER = GLU ? 1u : 2u;  // output tiles of a pair
+    const int lane = threadIdx.x & 63;
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4, aoff = a_lane_offset(lane);
+    const uint32_t steps = o.steps, t0 = t_begin + wave * PER;
+    if (t0 >= t_end) return;
+    const uint32_t pairs = (t_end - t0 + 4u * PER - 1u) / (4u * PER), total = pairs * steps;
+    const size_t sx_at = (size_t)steps * Kcfg<KIND>::P * A_TILE_STRIDE;
+
+    // fetches run ahead of the products through the pairs and their steps
+    uint32_t ft = 0, fT = t0;
+    uint4 hdr[2] = {};
+    auto heads = [&](uint32_t T, uint32_t t) {
+        if constexpr (KIND == HK_MIXED) {
+            hdr[0] = ldg(o.hdr + (min(T, a.n_row_tiles - 1u) * steps + t));
+            hdr[1] = ldg((GLU ? ou.hdr : o.hdr) + (min(GLU ? T : T + 1u, a.n_row_tiles - 1u) * steps + t));
+        }
+    };
+    Frag<KIND, 1> f[DEPTH][2];
+    auto advance = [&]() {
+        if (++ft == steps) {
+            ft = 0;
+            fT += 4u * PER;
+        }
+    };
+    auto fetch = [&](Frag<KIND, 1>(&x)[2]) {
+        const uint32_t Ta = min(fT, a.n_row_tiles - 1u), Tb = min(GLU ? fT : fT + 1u, a.n_row_tiles - 1u);
+        if constexpr (KIND == HK_MIXED) {
+            fetch_mixed<1>(o, hdr[0], lane, x[0], 0);
+            fetch_mixed<1>(GLU ? ou : o, hdr[1], lane, x[1], 0);
+            advance();
+            heads(fT, ft);  // the next fetch's headers, a step early
+        } else {
+            fetch_one<KIND, 1, true>(o, Ta, ft, lane, x[0], 0);
+            fetch_one<KIND, 1, true>(GLU ? ou : o, Tb, ft, lane, x[1], 0);
+            advance();
+        }
+    };
+    heads(fT, 0);
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(f[d]);
+
+    float acc[NP][2], fin = 0.0f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) acc[p][0] = acc[p][1] = 0.0f;
+    uint32_t t = 0, T = t0;
+    auto step = [&](uint32_t i, const Frag<KIND, 1>(&cur)[2], Frag<KIND, 1>(&nxt)[2]) {
+        fetch(nxt);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const uint8_t* img = lds + p * img_bytes;
+            const float* SX = reinterpret_cast<const float*>(img + sx_at);
+            compute_step<KIND, 1>(cur[0], t, ImageA{img, aoff}, SX, (int)q, &acc[p][0]);
+            compute_step<KIND, 1>(cur[1], t, ImageA{img, aoff}, SX, (int)q, &acc[p][1]);
+        }
+        if (++t < steps) return;
+        // the pair is done: lane (m, q) stores row m of position q
+        t = 0;
+        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const float v0 = tile_row_sum(acc[p][0]), v1 = tile_row_sum(acc[p][1]);
+            if (q == (uint32_t)p) s0 = v0, s1 = v1;
+            acc[p][0] = acc[p][1] = 0.0f;
+        }
+        const uint32_t pos = first + q;
+        if (q < (uint32_t)NP && pos < last) {
+            const bool nan = exps[q] == ROWS_EXP_BAD;
+            float v[2] = {GLU ? rows_silu(s0) * s1 : s0, s1};
+#pragma unroll
+            for (uint32_t r = 0; r < PER; ++r) {
+                const uint32_t row = 16u * (T + r) + m;
+                if (nan) v[r] = __builtin_nanf("");
+                if (T + r < t_end && row < a.rows) {
+                    fin = __builtin_fmaf(v[r], 0.0f, fin);
+                    const size_t at = (size_t)pos * a.y_stride + row;
+                    if (a.y_type == HK_T_F32) static_cast<float*>(a.y)[at] = v[r];
+                    else static_cast<uint16_t*>(a.y)[at] = a.y_type == HK_T_BF16 ? f32_to_bf16_bits(v[r]) : f32_to_f16_bits(v[r]);
+                }
+            }
+        }
+        T += 4u * PER;
+        (void)i;
+    };
+    uint32_t i = 0;
+    for (; i + DEPTH <= total; i += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) step(i + d, f[d], f[(d + DEPTH - 1) % DEPTH]);
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d)
+        if (i + d < total) step(i + d, f[d], f[(d + DEPTH - 1) % DEPTH]);
+    if (__ballot(fin != fin) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
+}
+
+// block_tiles: output row tiles of a workgroup; tile_rows: positions of a tile.
+template <int KIND, int FORM>
+__global__ void __launch_bounds__(256) rows_vec_kernel(RowsArgs a, uint32_t block_tiles, uint32_t img_bytes) {
+    extern __shared__ __align__(16) uint8_t lds[];  // tile_rows images
+    __shared__ int32_t exps[4];
+    uint32_t tile, block, group, first, last;
+    rows_item(a, &tile, &block);
+    if (!rows_positions<FORM, 4>(a, tile, &group, &first, &last)) return;
+    const uint32_t np = last - first, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t p = 0; p < np; ++p) {
+        bool bad;
+        const uint32_t r = rows_source(a, first + p, &bad);
+        copy16_to_lds<4>(reinterpret_cast<uint4*>(lds + p * img_bytes),
+                         reinterpret_cast<const uint4*>(a.ws.img + (size_t)r * img_bytes), img_bytes / 16u, threadIdx.x, 256u);
+        if (threadIdx.x == 0) {
+            exps[p] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
+            if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
+        }
+    }
+    const OrganView o = rows_view(a.organs, group);
+    const OrganView ou = FORM == ROWS_GLU ? rows_view(a.up, group) : o;
+    const uint32_t tb = block * block_tiles, te = min(tb + block_tiles, a.n_row_tiles);
+    __syncthreads();
+    if (np == 1u) rows_vec<KIND, 1, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
+    else if (np == 2u) rows_vec<KIND, 2, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
+    else rows_vec<KIND, 4, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
+}
+
+template <int KIND, int FORM>
+hipError_t rows_vec_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
+    const uint32_t img = (uint32_t)rows_vec_image_bytes(KIND, a.cols);
+    a.tiles = a.ws.max_tiles;
+    a.row_blocks = (a.n_row_tiles + sh.block_tiles - 1u) / sh.block_tiles;
+    const uint64_t grid = (a.tiles < ROWS_XCD_TILES ? (uint64_t)a.tiles : ((uint64_t)a.tiles + 7u) / 8u * 8u) * a.row_blocks;
+    if (grid == 0) return hipSuccess;
+    if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
+    auto* k = rows_vec_kernel<KIND, FORM>;
+    hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), (size_t)sh.tile_rows * img, s, a, sh.block_tiles, img);
+    return hipGetLastError();
+}
+
+template <int KIND>
+hipError_t launch_rows_vec_image_kind(const void* x, int type, size_t stride, uint32_t n, uint32_t cols, const RowsWs& ws,
+                                      const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
+                                      uint32_t* status, hipStream_t s) {
+    const bool vec = stride % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (type == HK_T_F32 ? 16 : 8) == 0;
+    hipLaunchKernelGGL(rows_vec_image_kernel<KIND>, dim3(n + 1u), dim3(256), 0, s, x, type, stride, n, cols, vec, ws, offsets,
+                       groups, n_pos, tile_rows, status);
+    return hipGetLastError();
+}
+
 // ------------------------------------------------------------------ launch
 
 template <int KIND, int WP, int XP, int MT, int FORM, bool TILE>
@@ -635,6 +849,8 @@ hipError_t rows_form(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
 // Binary weights are exact in one plane.
 template <int KIND>
 hipError_t launch_rows_kind(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
+    if (sh.vec)
+        return sh.form == ROWS_GLU ? rows_vec_go<KIND, ROWS_GLU>(sh, a, s) : rows_vec_go<KIND, ROWS_PLAIN>(sh, a, s);
     constexpr int W2 = KIND == HK_BIN ? 1 : 2;
     if (sh.xp == 2) return rows_form<KIND, W2, 2>(sh, a, s);
     if (sh.wp == 2) return rows_form<KIND, W2, 1>(sh, a, s);

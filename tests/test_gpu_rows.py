@@ -108,7 +108,9 @@ def _exact_grouped(xe, off, src, ws, x_type, y_type):
 
 
 COUNTS = {
-    # mean rows a group: up to 16 the split kernel, up to 64 the tile kernel with 64 rows, beyond with 128 (64 for f32 -> f32)
+    # mean rows a group: up to 4 the int8 engine, up to 16 the split kernel, up to 64 the tile kernel with 64 rows, beyond with 128
+    # (64 where two planes are needed); a few tiles alone take the split kernel
+    "ones": [1, 0, 2, 3, 4, 5, 9, 0, 1, 1],
     "few": [0, 1, 2, 15, 16, 17, 0, 0, 33, 1],
     "mid": [20, 0, 64, 65, 1, 130],
     "many": [129, 0, 257, 1, 300],
@@ -214,21 +216,26 @@ def test_swiglu_gathered(ctx, oracle, kind, rows, cols, tokens, per_row, groups,
     assert np.all(got[off[-1]:] == 5.0)
 
 
-def test_rows_do_not_depend_on_each_other(ctx, oracle):
-    """A row's bits are the same alone in its group and among others of one launch shape."""
+@pytest.mark.parametrize("n", [1, 3, 4, 16, 40, 300])
+def test_rows_do_not_depend_on_each_other(ctx, oracle, n):
+    """A row's bits are the same whatever the other rows of the call hold, and on every call."""
     from hawking_amd.organs import OrganSet
     from hawking_amd.rows import GroupedGemm
     rows, cols = 64, 384
-    w = R.make_organ(ctx, oracle, "q4", rows, cols, 3000)[0]
-    v = np.random.default_rng(1).standard_normal((16, cols))
-    for n in (1, 16):
-        plan, _, _ = _plan(ctx, [n])
-        x, _, _ = R.rows_on(ctx, v[:n], "f32")
+    s = OrganSet(ctx, [R.make_organ(ctx, oracle, "q4", rows, cols, 3000)[0]])
+    rng = np.random.default_rng(1)
+    v = rng.standard_normal((n, cols))
+    plan, _, _ = _plan(ctx, [n])
+    gemm = GroupedGemm(ctx, s, n, "f32", "f32")
+    seen = []
+    for other in (1.0, 1e6, 1e-6, 1.0):
+        w = v * other
+        w[0] = v[0]
+        x, _, _ = R.rows_on(ctx, w, "f32")
         y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
-        GroupedGemm(ctx, OrganSet(ctx, [w]), n, "f32", "f32")(x, plan, y)
-        first = R.read_rows(yb, y)[0][0] if n == 1 else first
-        last = R.read_rows(yb, y)[0]
-    assert np.array_equal(first, last[0])
+        gemm(x, plan, y)
+        seen.append(R.read_rows(yb, y)[0])
+    assert all(np.array_equal(seen[0][0], r[0]) for r in seen) and np.array_equal(seen[0], seen[3])
 
 
 @pytest.mark.parametrize("x_type", ["bf16", "f32", "f16"])
