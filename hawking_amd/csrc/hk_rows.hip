@@ -6,91 +6,114 @@ namespace hk {
 
 // ------------------------------------------------------------------ row images
 
-// Rows of x -> image rows (hk_rows.h), TPR threads a row; the last block makes
-// the product's tiles instead.  A row's maximum is taken first: up to four
-// chunks a thread stay in registers, more are read again (from the caches).
-template <int TYPE, int PLANES, int TPR>
+// What a row's maximum says: its exponent, or ROWS_EXP_BAD.
+__device__ __forceinline__ int32_t row_exp(float m) {
+    if (!isfinite(m)) return ROWS_EXP_BAD;
+    int e = 0;
+    if (m > 0.0f) (void)frexpf(m, &e);
+    return m > 0.0f ? 14 - e : 0;
+}
+// max |e| of a chunk, infinity if a value is not finite (fmaxf would drop a NaN).
+__device__ __forceinline__ float chunk_max(const float* e) {
+    float m = 0.0f, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m = fmaxf(m, fabsf(e[i]));
+        s = __builtin_fmaf(e[i], 0.0f, s);
+    }
+    return s != s ? INFINITY : m;
+}
+
+// Rows of x -> image rows (hk_rows.h); the last block makes the product's tiles
+// instead.  A row's maximum is taken first, from the chunks that then are
+// written: four a thread stay in registers, more are read again (from the
+// caches).  ROWS = 0: a workgroup a row.  Else: a wave ROWS rows at once, whose
+// 64 * 4 / ROWS chunks are one round of loads (a row of 512 columns alone is one
+// load a lane, and its latency the cost: 40960 of them 30 us, four at once 19).
+template <int TYPE, int PLANES, int ROWS>
 __global__ void __launch_bounds__(256) rows_image_kernel(const void* x, size_t stride, uint32_t n, uint32_t cols, int kind,
                                                          uint32_t chunks, bool vec, RowsWs ws, const int32_t* offsets,
                                                          uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
                                                          uint32_t* status) {
-    constexpr int NC = 4;
-    __shared__ uint32_t pre[256];
+    constexpr int R = ROWS ? ROWS : 1, NC = 4 / R;
+    constexpr uint32_t TPR = ROWS ? 64 : 256;
+    __shared__ RowsTileMap map;
     if (offsets && blockIdx.x == gridDim.x - 1u) {
-        rows_tiles(ws, offsets, groups, n_pos, tile_rows, pre);
+        rows_tiles(ws, offsets, groups, n_pos, tile_rows, map);
         return;
     }
-    const uint32_t row = blockIdx.x * (256u / TPR) + threadIdx.x / TPR, me = threadIdx.x % TPR;
-    if (TPR < 256 && row >= n) return;  // a whole wave
-    const size_t base = (size_t)row * stride;
+    const uint32_t row0 = ROWS ? (blockIdx.x * 4u + (threadIdx.x >> 6)) * R : blockIdx.x, me = threadIdx.x % TPR;
+    if (row0 >= n) return;  // a whole wave
     const uint32_t apart = (kind == HK_BIN || kind == HK_MIXED) ? 16u : 4u;
-    auto load = [&](uint32_t ch, float* v) {
+    auto load = [&](uint32_t row, uint32_t ch, float* v) {
         const uint32_t c = rows_chunk_cols(kind, ch).c0;  // columns come in whole 32s
-        if (ch < chunks && c < cols) {
-            row_load4(TYPE, x, base + c, vec, v);
-            row_load4(TYPE, x, base + c + apart, vec, v + 4);
+        if (row < n && ch < chunks && c < cols) {
+            row_load4(TYPE, x, (size_t)row * stride + c, vec, v);
+            row_load4(TYPE, x, (size_t)row * stride + c + apart, vec, v + 4);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = 0.0f;
         }
     };
-    float v[NC][8];
-    float m = 0.0f;
+    float v[R][NC][8], m[R];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) load(me + (uint32_t)i * TPR, v[i]);
-    auto top = [&](const float* e) {
-        float s = 0.0f;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m = fmaxf(m, fabsf(e[i]));
-            s += e[i] - e[i];  // NaN for an infinity or a NaN, which fmaxf would drop
+        for (int i = 0; i < NC; ++i) load(row0 + r, me + (uint32_t)i * TPR, v[r][i]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) m[r] = fmaxf(m[r], chunk_max(v[r][i]));
+    }
+    if constexpr (!ROWS)
+        for (uint32_t ch = me + NC * TPR; ch < chunks; ch += TPR) {
+            float e[8];
+            load(row0, ch, e);
+            m[0] = fmaxf(m[0], chunk_max(e));
         }
-        if (s != s) m = INFINITY;
-    };
+    int32_t E[R];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) top(v[i]);
-    for (uint32_t ch = me + NC * TPR; ch < chunks; ch += TPR) {
-        float e[8];
-        load(ch, e);
-        top(e);
-    }
-    m = wave_max(m);
-    if constexpr (TPR == 256) {
-        float* red = reinterpret_cast<float*>(pre);
-        if ((threadIdx.x & 63u) == 0u) red[threadIdx.x >> 6] = m;
+    for (int r = 0; r < R; ++r) m[r] = wave_max(m[r]);
+    if constexpr (!ROWS) {
+        float* red = reinterpret_cast<float*>(map.wsum);
+        if ((threadIdx.x & 63u) == 0u) red[threadIdx.x >> 6] = m[0];
         __syncthreads();
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        m[0] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     }
-    const bool bad = !isfinite(m);
-    int e2 = 0;
-    if (!bad && m > 0.0f) (void)frexpf(m, &e2);
-    const int E = (!bad && m > 0.0f) ? 14 - e2 : 0;
-    if (me == 0) {
-        ws.exps[row] = bad ? ROWS_EXP_BAD : E;
-        if (bad) atomicOr(status, ROWS_ERR_NONFINITE);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        E[r] = row_exp(m[r]);
+        if (me == 0 && row0 + r < n) {
+            ws.exps[row0 + r] = E[r];
+            if (E[r] == ROWS_EXP_BAD) atomicOr(status, ROWS_ERR_NONFINITE);
+        }
     }
-    uint8_t* out = ws.img + (size_t)row * chunks * (16u * PLANES);
-    auto put = [&](uint32_t ch, const float* e) {
-        if (ch >= chunks) return;
+    auto put = [&](int r, uint32_t ch, const float* e) {
+        if (ch >= chunks || row0 + r >= n) return;
+        const bool bad = E[r] == ROWS_EXP_BAD;
         hk_f16x8 h, l;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             // element order: pairs (k, k + 4) of what was loaded; Q8 takes the columns in order
-            const float f = bad ? 0.0f : ldexpf(kind == HK_Q8 ? e[k] : e[(k >> 1) + 4 * (k & 1)], E);
+            const float f = bad ? 0.0f : ldexpf(kind == HK_Q8 ? e[k] : e[(k >> 1) + 4 * (k & 1)], E[r]);
             h[k] = (_Float16)f;
             if constexpr (PLANES == 2) l[k] = (_Float16)(f - (float)h[k]);
         }
-        uint8_t* p = out + (size_t)(ch >> 4) * (256u * PLANES) + (ch & 15u) * 16u;
+        uint8_t* p = ws.img + (size_t)(row0 + r) * chunks * (16u * PLANES) + (size_t)(ch >> 4) * (256u * PLANES) + (ch & 15u) * 16u;
         *reinterpret_cast<hk_f16x8*>(p) = h;
         if constexpr (PLANES == 2) *reinterpret_cast<hk_f16x8*>(p + 256u) = l;
     };
 #pragma unroll
-    for (int i = 0; i < NC; ++i) put(me + (uint32_t)i * TPR, v[i]);
-    for (uint32_t ch = me + NC * TPR; ch < chunks; ch += TPR) {
-        float e[8];
-        load(ch, e);
-        put(ch, e);
-    }
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) put(r, me + (uint32_t)i * TPR, v[r][i]);
+    if constexpr (!ROWS)
+        for (uint32_t ch = me + NC * TPR; ch < chunks; ch += TPR) {
+            float e[8];
+            load(row0, ch, e);
+            put(0, ch, e);
+        }
 }
 
 template <int TYPE, int PLANES>
@@ -100,14 +123,19 @@ static hipError_t image_go(const void* x, size_t stride, uint32_t n, uint32_t co
     const uint32_t chunks = rows_stages(kind, cols) * 16u, extra = offsets ? 1u : 0u;
     const size_t es = TYPE == HK_T_F32 ? 4 : 2;
     const bool vec = stride % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * es) == 0;
-    // a wave a row where that holds the row in registers and fills the device
-    if (chunks <= 256u && n >= 2048u)
-        hipLaunchKernelGGL((rows_image_kernel<TYPE, PLANES, 64>), dim3((n + 3u) / 4u + extra), dim3(256), 0, s, x, stride, n,
-                           cols, kind, chunks, vec, ws, offsets, groups, n_pos, tile_rows, status);
-    else
-        hipLaunchKernelGGL((rows_image_kernel<TYPE, PLANES, 256>), dim3(n + extra), dim3(256), 0, s, x, stride, n, cols, kind,
-                           chunks, vec, ws, offsets, groups, n_pos, tile_rows, status);
-    return hipGetLastError();
+    // a wave one, two or four rows where that holds them in registers and fills the device
+    const uint32_t rows = n < 2048u || chunks > 256u ? 0u : chunks <= 64u ? 4u : chunks <= 128u ? 2u : 1u;
+    auto go = [&](auto* kernel, uint32_t blocks) {
+        hipLaunchKernelGGL(kernel, dim3(blocks + extra), dim3(256), 0, s, x, stride, n, cols, kind, chunks, vec, ws, offsets,
+                           groups, n_pos, tile_rows, status);
+        return hipGetLastError();
+    };
+    switch (rows) {
+    case 4: return go(rows_image_kernel<TYPE, PLANES, 4>, (n + 15u) / 16u);
+    case 2: return go(rows_image_kernel<TYPE, PLANES, 2>, (n + 7u) / 8u);
+    case 1: return go(rows_image_kernel<TYPE, PLANES, 1>, (n + 3u) / 4u);
+    default: return go(rows_image_kernel<TYPE, PLANES, 0>, n);
+    }
 }
 
 hipError_t launch_rows_image(const void* x, int x_type, size_t x_stride, uint32_t n, uint32_t cols, int kind, int planes,

@@ -34,44 +34,53 @@ __device__ __forceinline__ void row_load4(int type, const void* x, size_t at, bo
 }
 
 // The positions [first, last) of every group cut into tiles of tile_rows, in
-// group order.  One block; offsets outside [0, n] or out of order are clamped,
-// so whatever they hold a tile lies inside the positions.
+// group order, then tiles without positions up to max_tiles.  One block of 256
+// threads, 1024 groups a round.  Offsets outside [0, n] or out of order are
+// clamped, so whatever they hold a tile lies inside the positions.
+constexpr uint32_t ROWS_MAP_GROUPS = 1024;
+struct RowsTileMap {
+    uint32_t pre[ROWS_MAP_GROUPS], lo[ROWS_MAP_GROUPS], hi[ROWS_MAP_GROUPS], wsum[4];
+};
 __device__ inline void rows_tiles(const RowsWs& ws, const int32_t* offsets, uint32_t groups, uint32_t n, uint32_t tile_rows,
-                           uint32_t* pre) {
+                                  RowsTileMap& map) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    __shared__ uint32_t wsum[4], lo_s[256];
     uint32_t base = 0;
-    for (uint32_t g0 = 0; g0 < groups; g0 += 256u) {
-        const uint32_t g = g0 + tid;
-        uint32_t lo = 0, hi = 0;
-        if (g < groups) {
-            lo = min((uint32_t)max(offsets[g], 0), n);
-            hi = max(min((uint32_t)max(offsets[g + 1], 0), n), lo);
+    for (uint32_t g0 = 0; g0 < groups; g0 += ROWS_MAP_GROUPS) {
+        const uint32_t g = g0 + 4u * tid;
+        uint32_t at[5], c[4], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 5; ++i) at[i] = min((uint32_t)max(ldg(offsets + min(g + i, groups)), 0), n);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            c[i] = at[i + 1] > at[i] ? (at[i + 1] - at[i] + tile_rows - 1u) / tile_rows : 0u;
+            sum += c[i];
         }
-        const uint32_t c = (hi - lo + tile_rows - 1u) / tile_rows;
-        const uint32_t inc = wave_incl_scan(c);
+        const uint32_t inc = wave_incl_scan(sum);
         __syncthreads();  // the last round's readers are done
-        if (lane == 63u) wsum[wave] = inc;
-        lo_s[tid] = lo;
+        if (lane == 63u) map.wsum[wave] = inc;
         __syncthreads();
-        uint32_t before = 0, total = 0;
+        uint32_t before = inc - sum, total = 0;
 #pragma unroll
         for (uint32_t w = 0; w < 4; ++w) {
-            if (w < wave) before += wsum[w];
-            total += wsum[w];
+            if (w < wave) before += map.wsum[w];
+            total += map.wsum[w];
         }
-        pre[tid] = before + inc - c;  // tiles of the round before this group
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            map.pre[4u * tid + i] = before;  // tiles of the round before this group
+            map.lo[4u * tid + i] = at[i];
+            map.hi[4u * tid + i] = at[i + 1];
+            before += c[i];
+        }
         __syncthreads();
         for (uint32_t j = tid; j < total; j += 256u) {
-            // the last group that begins at or before tile j and has tiles: pre is ascending, empty groups share the next one's start
-            uint32_t a = 0, b = 256u;
-            while (b - a > 1u) {
-                const uint32_t mid = (a + b) / 2u;
-                if (pre[mid] <= j) a = mid; else b = mid;
-            }
-            const uint32_t first = lo_s[a] + (j - pre[a]) * tile_rows;
-            const uint32_t end = max(min((uint32_t)max(offsets[g0 + a + 1u], 0), n), lo_s[a]);
-            if (base + j < ws.max_tiles) ws.tiles[base + j] = RowsTile{g0 + a, first, min(first + tile_rows, end), 0u};
+            // the last group that begins at or before tile j (an empty group begins where the next one does)
+            uint32_t k = 0;
+#pragma unroll
+            for (uint32_t s = ROWS_MAP_GROUPS / 2u; s; s >>= 1)
+                if (map.pre[k + s] <= j) k += s;
+            const uint32_t first = map.lo[k] + (j - map.pre[k]) * tile_rows;
+            if (base + j < ws.max_tiles) ws.tiles[base + j] = RowsTile{g0 + k, first, min(first + tile_rows, map.hi[k]), 0u};
         }
         base += total;
     }

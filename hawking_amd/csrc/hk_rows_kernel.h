@@ -133,70 +133,102 @@ __device__ __forceinline__ void rows_each(F&& f) {
     }
 }
 
-// The adapters' part: acc (units of 2^-exps) is moved to the units of the
-// position's mid row and B_s mid is added for every slot s with positions in
-// the tile [first, last); the other positions' mid counts as zero.  T: the
-// RT row tiles of this wave; exps: this lane's position of every 16, updated.
+// The adapters' part.  Positions with an adapter (those before
+// offsets[slots]) are first moved from the units of their x row (2^-exps) to
+// those of their mid row; then B_s mid is added for the slots s with positions
+// in the tile [first, last) -- every kw-th of them where kw waves share the
+// sums, this wave beginning with the wk-th.  A position's mid row is read once;
+// for a slot that is not its own it counts as zero.  B comes RB slots at a time,
+// since a slot is one product and its latency is the cost.  T: the RT row tiles
+// of this wave; exps: this lane's position of every 16, updated.
 template <int MT, int RT>
 __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane,
-                                          int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
+                                          uint32_t wk, uint32_t kw, int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
+    constexpr int RB = RT == 2 ? 4 : 2;
     const RowsLora& L = a.lora;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
-    const size_t pitch = (size_t)L.kk_max * 64u * L.planes;
-    for (uint32_t s0 = 0; s0 < L.slots; s0 += 64u) {
-        const uint32_t sl = s0 + (uint32_t)lane;
-        uint32_t o0 = 0, o1 = 0;
-        if (sl < L.slots) {
-            o0 = min((uint32_t)max(L.offsets[sl], 0), a.n);
-            o1 = min((uint32_t)max(L.offsets[sl + 1], 0), a.n);
+    const uint32_t pitch = L.kk_max * 64u * L.planes;
+    const uint32_t grouped = min((uint32_t)max(L.offsets[L.slots], 0), a.n);
+    if (first >= grouped) return;
+    rows_each<MT>([&](auto mt) {
+        const uint32_t p = first + 16u * mt + m;
+        if (p < grouped) {
+            const int32_t g = L.mid_exps[p];
+            const bool nan = exps[mt] == ROWS_EXP_BAD || g == ROWS_EXP_BAD;
+            const int d = nan ? 0 : g - exps[mt];
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[mt][r][j] = ldexpf(acc[mt][r][j], d);
+            exps[mt] = nan ? ROWS_EXP_BAD : g;
         }
-        uint64_t hit = __ballot(o0 < last && o1 > first && o0 < o1);
-        while (hit) {
-            const int i = __builtin_ctzll(hit);
-            hit &= hit - 1;
-            const uint32_t s = s0 + (uint32_t)i;
-            const uint32_t lo = max(__builtin_amdgcn_readlane(o0, i), first), hi = min(__builtin_amdgcn_readlane(o1, i), last);
-            const uint32_t kk = min((L.tab[s].rank + 31u) / 32u, L.kk_max);
-            if (!kk) continue;
+    });
+    for (uint32_t k = 0; k < L.kk_max; ++k)
+        for (uint32_t pl = 0; pl < L.planes; ++pl) {
+            // opaque to the compiler: it would keep the MT rows' addresses in registers over the loops, and spill
+            uint32_t f = first;
+            asm volatile("" : "+s"(f));
+            uint4 mid[MT];
             rows_each<MT>([&](auto mt) {
-                const uint32_t p = first + 16u * mt + m;
-                if (p >= lo && p < hi) {
-                    const int32_t g = L.mid_exps[p];
-                    const bool nan = exps[mt] == ROWS_EXP_BAD || g == ROWS_EXP_BAD;
-                    const int d = nan ? 0 : g - exps[mt];
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[mt][r][j] = ldexpf(acc[mt][r][j], d);
-                    exps[mt] = nan ? ROWS_EXP_BAD : g;
-                }
+                const uint32_t p = min(f + 16u * mt + m, grouped - 1u);
+                mid[mt] = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)p * pitch + (pl * L.kk_max + k) * 64u + 16u * q));
             });
-            for (uint32_t k = 0; k < kk; ++k) {
-                // opaque to the compiler: it would keep the MT rows' addresses in registers over the loop, and spill
-                uint32_t f = first;
-                asm volatile("" : "+s"(f));
-                hk_f16x8 w[RT];
+            uint32_t seen = 0;  // slots of the tile so far
+            for (uint32_t s0 = 0; s0 < L.slots; s0 += 64u) {
+                const uint32_t sl = s0 + (uint32_t)lane;
+                uint32_t o0 = 0, o1 = 0, rank = 0;
+                if (sl < L.slots) {
+                    o0 = min((uint32_t)max(L.offsets[sl], 0), a.n);
+                    o1 = min((uint32_t)max(L.offsets[sl + 1], 0), a.n);
+                    rank = L.tab[sl].rank;
+                }
+                uint64_t hit = __ballot(o0 < last && o1 > first && o0 < o1 && rank > 32u * k);
+                while (hit) {
+                    uint32_t s[RB], lo[RB], hi[RB];
+                    int n = 0;
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
-                    w[r] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
-                                                            L.b + (((size_t)s * a.n_row_tiles + T[r]) * L.kk_max + k) * 1024u + 16u * (uint32_t)lane)));
-                for (uint32_t pl = 0; pl < L.planes; ++pl)
-                    rows_each<MT>([&](auto mt) {
-                        const uint32_t t0 = f + 16u * mt;
-                        if (t0 < hi && t0 + 16u > lo) {  // uniform
-                            const uint32_t p = t0 + m;
-                            const bool mine = p >= lo && p < hi;
-                            uint4 v = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)(mine ? p : lo) * pitch +
-                                                                         ((size_t)pl * L.kk_max + k) * 64u + 16u * q));
-                            if (!mine) v = make_uint4(0u, 0u, 0u, 0u);
-                            const hk_f16x8 x = __builtin_bit_cast(hk_f16x8, v);
-#pragma unroll
-                            for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(w[r], x, acc[mt][r]);
+                    for (int b = 0; b < RB; ++b) {
+                        // this wave's next slot, if any
+                        while (hit && seen % kw != wk) {
+                            hit &= hit - 1;
+                            ++seen;
                         }
-                    });
+                        s[b] = s0, lo[b] = hi[b] = 0;
+                        if (hit) {
+                            const int i = __builtin_ctzll(hit);
+                            hit &= hit - 1;
+                            ++seen;
+                            s[b] = s0 + (uint32_t)i;
+                            lo[b] = __builtin_amdgcn_readlane(o0, i);
+                            hi[b] = __builtin_amdgcn_readlane(o1, i);
+                            n = b + 1;
+                        }
+                    }
+                    hk_f16x8 w[RB][RT];
+#pragma unroll
+                    for (int b = 0; b < RB; ++b)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+                            w[b][r] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
+                                L.b + (((size_t)s[b] * a.n_row_tiles + T[r]) * L.kk_max + k) * 1024u + 16u * (uint32_t)lane)));
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        if (b >= n) break;
+                        rows_each<MT>([&](auto mt) {
+                            const uint32_t t0 = f + 16u * mt, p = t0 + m;
+                            if (t0 < hi[b] && t0 + 16u > lo[b]) {  // uniform
+                                const bool mine = p >= lo[b] && p < hi[b];
+                                const uint4 v = mid[mt];
+                                const hk_f16x8 x = __builtin_bit_cast(
+                                    hk_f16x8, make_uint4(mine ? v.x : 0u, mine ? v.y : 0u, mine ? v.z : 0u, mine ? v.w : 0u));
+#pragma unroll
+                                for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(w[b][r], x, acc[mt][r]);
+                            }
+                        });
+                    }
+                }
             }
         }
-    }
 }
 
 // Scales a tile's sums back and stores them; GLU: row tiles r and r + RT / 2
@@ -447,7 +479,7 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
     int32_t exps[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) exps[mt] = map[16 * mt + m].exp;
-    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
+    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, 0, 1, exps, acc);
     // (the last stage ended with a barrier: its buffers are free)
     rows_store_tile<MT, RT, GLU>(a, first, last, T0, lane, map, lds + wave * ROWS_OUT_BYTES, exps, acc);
 }
@@ -566,6 +598,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
             for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
         }
     }
+    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, wk, kw, exps, acc);
     if (kw > 1) {
         // part[wave - wr - 1]: the waves that are not their pair's first
         if (wk) {
@@ -583,7 +616,6 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
                 for (int r = 0; r < RT; ++r) acc[mt][r] += part[wave + k - wr - 1u][mt * RT + r][lane];
     }
     if (T0 >= a.n_row_tiles) return;
-    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, exps, acc);
     rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
 }
 
@@ -606,10 +638,10 @@ __global__ void __launch_bounds__(256) rows_vec_image_kernel(const void* x, int 
                                                              uint32_t n_pos, uint32_t tile_rows, uint32_t* status) {
     constexpr uint32_t SC = Kcfg<KIND>::STEP_COLS, UNIT_FLOATS = Kcfg<KIND>::SXW, PART = 2048;
     __shared__ __align__(16) float xs[PART];
-    __shared__ uint32_t pre[256];
+    __shared__ RowsTileMap map;
     __shared__ uint32_t bad_s;
     if (blockIdx.x == gridDim.x - 1u) {
-        rows_tiles(ws, offsets, groups, n_pos, tile_rows, pre);
+        rows_tiles(ws, offsets, groups, n_pos, tile_rows, map);
         return;
     }
     const uint32_t row = blockIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -648,19 +680,19 @@ __global__ void __launch_bounds__(256) rows_vec_image_kernel(const void* x, int 
     }
 }
 
-// NP positions (images at lds + p bytes) x this wave's row tile pairs.
+// NP positions (images at lds + p img_bytes, copied there after the first
+// weights were asked for) x this wave's row tile pairs.
 template <int KIND, int NP, int FORM>
 __device__ __forceinline__ void rows_vec(const RowsArgs& a, const OrganView& o, const OrganView& ou, uint32_t first,
-                                         uint32_t last, uint32_t t_begin, uint32_t t_end, uint32_t wave, const uint8_t* lds,
-                                         uint32_t img_bytes, const int32_t* exps) {
+                                         uint32_t last, uint32_t t_begin, uint32_t t_end, uint32_t wave, uint8_t* lds,
+                                         uint32_t img_bytes, int32_t* exps) {
     constexpr bool GLU = FORM == ROWS_GLU;
     constexpr int DEPTH = 3;
     constexpr uint32_t PER = GLU ? 1u : 2u;  // output tiles of a pair
     const int lane = threadIdx.x & 63;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4, aoff = a_lane_offset(lane);
     const uint32_t steps = o.steps, t0 = t_begin + wave * PER;
-    if (t0 >= t_end) return;
-    const uint32_t pairs = (t_end - t0 + 4u * PER - 1u) / (4u * PER), total = pairs * steps;
+    const uint32_t pairs = t0 < t_end ? (t_end - t0 + 4u * PER - 1u) / (4u * PER) : 0u, total = pairs * steps;
     const size_t sx_at = (size_t)steps * Kcfg<KIND>::P * A_TILE_STRIDE;
 
     // fetches run ahead of the products through the pairs and their steps
@@ -695,6 +727,18 @@ __device__ __forceinline__ void rows_vec(const RowsArgs& a, const OrganView& o, 
     heads(fT, 0);
 #pragma unroll
     for (int d = 0; d < DEPTH - 1; ++d) fetch(f[d]);
+
+    for (uint32_t p = 0; p < last - first; ++p) {
+        bool bad;
+        const uint32_t r = rows_source(a, first + p, &bad);
+        copy16_to_lds<4>(reinterpret_cast<uint4*>(lds + p * img_bytes),
+                         reinterpret_cast<const uint4*>(a.ws.img + (size_t)r * img_bytes), img_bytes / 16u, threadIdx.x, 256u);
+        if (threadIdx.x == 0) {
+            exps[p] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
+            if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
+        }
+    }
+    __syncthreads();
 
     float acc[NP][2], fin = 0.0f;
 #pragma unroll
@@ -758,20 +802,9 @@ __global__ void __launch_bounds__(256) rows_vec_kernel(RowsArgs a, uint32_t bloc
     rows_item(a, &tile, &block);
     if (!rows_positions<FORM, 4>(a, tile, &group, &first, &last)) return;
     const uint32_t np = last - first, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t p = 0; p < np; ++p) {
-        bool bad;
-        const uint32_t r = rows_source(a, first + p, &bad);
-        copy16_to_lds<4>(reinterpret_cast<uint4*>(lds + p * img_bytes),
-                         reinterpret_cast<const uint4*>(a.ws.img + (size_t)r * img_bytes), img_bytes / 16u, threadIdx.x, 256u);
-        if (threadIdx.x == 0) {
-            exps[p] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
-            if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
-        }
-    }
     const OrganView o = rows_view(a.organs, group);
     const OrganView ou = FORM == ROWS_GLU ? rows_view(a.up, group) : o;
     const uint32_t tb = block * block_tiles, te = min(tb + block_tiles, a.n_row_tiles);
-    __syncthreads();
     if (np == 1u) rows_vec<KIND, 1, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
     else if (np == 2u) rows_vec<KIND, 2, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
     else rows_vec<KIND, 4, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
