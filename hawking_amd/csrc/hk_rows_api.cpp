@@ -75,7 +75,7 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     sh.tile_rows = 16u * sh.mt;
     // columns over as many waves as have a superstep each
     const uint32_t supers = (kind == HK_BIN || kind == HK_MIXED) ? stages / 4u : stages;
-    sh.kw = supers >= 4 ? 4 : supers >= 2 ? 2 : 1;
+    sh.kw = supers >= 8 ? 8 : supers >= 4 ? 4 : supers >= 2 ? 2 : 1;
     return sh;
 }
 

@@ -144,7 +144,7 @@ __device__ __forceinline__ void rows_each(F&& f) {
 template <int MT, int RT>
 __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane,
                                           uint32_t wk, uint32_t kw, int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
-    constexpr int RB = RT == 2 ? 4 : 2;
+    constexpr int RB = RT == 4 ? 2 : 8 / RT;
     const RowsLora& L = a.lora;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
     const uint32_t pitch = L.kk_max * 64u * L.planes;
@@ -507,19 +507,21 @@ __global__ void __launch_bounds__(256, MT == 4 && WP == 1 && XP == 1 && KIND != 
 
 // ------------------------------------------------------------------ few rows a group: columns split over the waves
 
-// A workgroup of four waves: 16 MT positions x (4 / kw) pairs of row tiles;
-// kw waves share a pair, wave w of them taking supersteps w, w + kw, ... and
-// their sums are added in LDS in wave order.  Such calls are bound by the
-// weight stream and its latency: the image is read straight from L2 (each
-// wave's reads equal its weights' decoded size), without LDS or barriers in
-// the loop, and many small workgroups keep the loads in flight.
-template <int KIND, int WP, int XP, int MT, int FORM>
-__global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsArgs a, uint32_t kw) {
-    constexpr int RT = 2, BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
+// A workgroup of eight waves: 16 MT positions x (8 / kw) sets of RT row tiles
+// (SwiGLU: one of the gate, one of the up organ); kw waves share a set, wave w
+// of them taking supersteps w, w + kw, ... and their sums are added in LDS in
+// wave order.  Such calls are bound by the weight stream and its latency: the
+// image is read straight from L2 (a product ahead, the weights a superstep
+// ahead), without LDS or barriers in the loop.
+constexpr uint32_t ROWS_SPLIT_WAVES = 8;
+template <int KIND, int WP, int XP, int MT, int FORM, int RT>
+__global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsArgs a, uint32_t kw) {
+    constexpr int BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
     constexpr bool GLU = FORM == ROWS_GLU;
-    __shared__ hk_f32x4 part[3][MT * RT][64];
+    extern __shared__ __align__(16) uint8_t lds[];
+    hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [8 - 8 / kw][MT * RT][64]
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = threadIdx.x >> 6, wk = wave % kw, wr = wave / kw;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave % kw, wr = wave / kw;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
 
     uint32_t tile, block, group, first, last;
@@ -527,31 +529,11 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
     if (!rows_positions<FORM, BM>(a, tile, &group, &first, &last)) return;
     const OrganView o = rows_view(a.organs, group);
     const OrganView ou = GLU ? rows_view(a.up, group) : o;
-    const uint32_t T0 = (block * (4u / kw) + wr) * (GLU ? RT / 2 : RT);
+    const uint32_t T0 = (block * (ROWS_SPLIT_WAVES / kw) + wr) * (GLU ? RT / 2 : RT);
     uint32_t T[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) T[r] = min(T0 + (uint32_t)(GLU ? r % (RT / 2) : r), a.n_row_tiles - 1u);
     auto view = [&](int r) -> const OrganView& { return (GLU && r >= RT / 2) ? ou : o; };
-
-    const size_t pitch = (size_t)a.stages * 256u * XP;
-    const uint8_t* xs[MT];
-    int32_t exps[MT];
-    bool any_bad = false;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        bool bad = false;
-        const uint32_t r = rows_source(a, min(first + 16u * mt + m, last - 1u), &bad);
-        xs[mt] = a.ws.img + (size_t)r * pitch + 16u * q;
-        exps[mt] = bad ? ROWS_EXP_BAD : a.ws.exps[r];
-        any_bad |= bad;
-    }
-    if (__ballot(any_bad) && lane == 0) atomicOr(a.status, ROWS_ERR_ROUTE);
-
-    hk_f32x4 acc[MT][RT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
 
     const uint32_t n_super = a.stages / STG;
     uint4 hdr[RT] = {};
@@ -566,46 +548,68 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
 #pragma unroll
         for (int r = 0; r < RT; ++r) rows_fetch<KIND>(view(r), T[r], min(t, n_super - 1u), lane, hdr[r], w[r]);
     };
-    if (wk < n_super) {
-        heads(wk);
-        w_load(wk, cur);
-        heads(wk + kw);
-        for (uint32_t t = wk; t < n_super; t += kw) {
-            w_load(t + kw, nxt);
-            heads(t + 2u * kw);
+    heads(wk);
+    w_load(wk, cur);
+    heads(wk + kw);
+
+    const size_t pitch = (size_t)a.stages * 256u * XP;
+    const uint8_t* xs[MT];
+    int32_t exps[MT];
+    uint32_t src[MT];
+    bool bad[MT], any_bad = false;
 #pragma unroll
-            for (int st = 0; st < STG; ++st) {
-                const size_t off = (size_t)(t * STG + st) * (256u * XP);
+    for (int mt = 0; mt < MT; ++mt) src[mt] = rows_source(a, min(first + 16u * mt + m, last - 1u), &bad[mt]);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    hk_f16x8 x[MT][XP];
+    for (int mt = 0; mt < MT; ++mt) {
+        xs[mt] = a.ws.img + (size_t)src[mt] * pitch + 16u * q;
+        any_bad |= bad[mt];
+    }
+    hk_f16x8 x[2][MT][XP];
+    auto x_load = [&](uint32_t s, int u, hk_f16x8(&v)[MT][XP]) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int p = 0; p < XP; ++p)
-                            x[mt][p] = __builtin_bit_cast(
-                                hk_f16x8, ldg(reinterpret_cast<const uint4*>(xs[mt] + off + 256u * p + 64u * u)));
+            for (int p = 0; p < XP; ++p)
+                v[mt][p] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
+                                                            xs[mt] + (size_t)min(s, a.stages - 1u) * (256u * XP) + 256u * p + 64u * u)));
+    };
+    x_load(wk * STG, 0, x[0]);
+    // (read after the operands, so that they do not wait for it)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        hk_f16x8 wh, wl;
-                        rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
+    for (int mt = 0; mt < MT; ++mt) exps[mt] = bad[mt] ? ROWS_EXP_BAD : a.ws.exps[src[mt]];
+    if (__ballot(any_bad) && lane == 0) atomicOr(a.status, ROWS_ERR_ROUTE);
+
+    hk_f32x4 acc[MT][RT];
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[mt], acc[mt][r]);
-                    }
-                }
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t t = wk; t < n_super; t += kw) {
+        w_load(t + kw, nxt);
+        heads(t + 2u * kw);
+        rows_each<STG * 4>([&](auto i) {
+            constexpr int st = i / 4, u = i % 4;
+            // the next product's image: of this stage, the next one, or this wave's next superstep
+            x_load(u < 3 ? t * STG + st : st < STG - 1 ? t * STG + st + 1u : (t + kw) * STG, (u + 1) % 4, x[(u + 1) & 1]);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                hk_f16x8 wh, wl;
+                rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[u & 1][mt], acc[mt][r]);
             }
+        });
 #pragma unroll
-            for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
-        }
+        for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
     }
     if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, wk, kw, exps, acc);
     if (kw > 1) {
-        // part[wave - wr - 1]: the waves that are not their pair's first
+        // part[wave - wr - 1]: the waves that are not their set's first
         if (wk) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) part[wave - wr - 1u][mt * RT + r][lane] = acc[mt][r];
+                for (int r = 0; r < RT; ++r) part[((wave - wr - 1u) * (MT * RT) + mt * RT + r) * 64u + lane] = acc[mt][r];
         }
         __syncthreads();
         if (wk) return;
@@ -613,7 +617,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 4 : 2) rows_split_kernel(RowsAr
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) acc[mt][r] += part[wave + k - wr - 1u][mt * RT + r][lane];
+                for (int r = 0; r < RT; ++r) acc[mt][r] += part[((wave + k - wr - 1u) * (MT * RT) + mt * RT + r) * 64u + lane];
     }
     if (T0 >= a.n_row_tiles) return;
     rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
@@ -810,17 +814,23 @@ __global__ void __launch_bounds__(256) rows_vec_kernel(RowsArgs a, uint32_t bloc
     else rows_vec<KIND, 4, FORM>(a, o, ou, first, last, tb, te, wave, lds, img_bytes, exps);
 }
 
+template <class Kernel, class... More>
+hipError_t rows_launch(Kernel* kernel, uint32_t tiles, uint32_t per, uint32_t threads, size_t lds, RowsArgs& a, hipStream_t s,
+                       More... more) {
+    a.tiles = tiles;
+    a.row_blocks = (a.n_row_tiles + per - 1u) / per;
+    const uint64_t grid = (tiles < ROWS_XCD_TILES ? (uint64_t)tiles : ((uint64_t)tiles + 7u) / 8u * 8u) * a.row_blocks;
+    if (grid == 0) return hipSuccess;
+    if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), lds, s, a, more...);
+    return hipGetLastError();
+}
+
 template <int KIND, int FORM>
 hipError_t rows_vec_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
     const uint32_t img = (uint32_t)rows_vec_image_bytes(KIND, a.cols);
-    a.tiles = a.ws.max_tiles;
-    a.row_blocks = (a.n_row_tiles + sh.block_tiles - 1u) / sh.block_tiles;
-    const uint64_t grid = (a.tiles < ROWS_XCD_TILES ? (uint64_t)a.tiles : ((uint64_t)a.tiles + 7u) / 8u * 8u) * a.row_blocks;
-    if (grid == 0) return hipSuccess;
-    if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
-    auto* k = rows_vec_kernel<KIND, FORM>;
-    hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), (size_t)sh.tile_rows * img, s, a, sh.block_tiles, img);
-    return hipGetLastError();
+    return rows_launch(rows_vec_kernel<KIND, FORM>, a.ws.max_tiles, sh.block_tiles, 256u, (size_t)sh.tile_rows * img, a, s,
+                       sh.block_tiles, img);
 }
 
 template <int KIND>
@@ -835,36 +845,29 @@ hipError_t launch_rows_vec_image_kind(const void* x, int type, size_t stride, ui
 
 // ------------------------------------------------------------------ launch
 
-template <int KIND, int WP, int XP, int MT, int FORM, bool TILE>
-hipError_t rows_go(const RowsShape& sh, RowsArgs a, hipStream_t s) {
-    constexpr uint32_t out_tiles = FORM == ROWS_GLU ? 2u : 1u;  // tiles per output tile
+template <int KIND, int WP, int XP, int MT, int FORM>
+hipError_t rows_go_tile(RowsArgs a, hipStream_t s) {
     const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles;
-    const uint32_t per = TILE ? 16u / out_tiles : 4u / sh.kw * 2u / out_tiles;
-    a.row_blocks = (a.n_row_tiles + per - 1u) / per;
-    a.tiles = tiles;
-    const uint64_t grid = (tiles < ROWS_XCD_TILES ? (uint64_t)tiles : ((uint64_t)tiles + 7u) / 8u * 8u) * a.row_blocks;
-    if (grid == 0) return hipSuccess;
-    if (grid > 0x7FFFFFFFull) return hipErrorInvalidConfiguration;
-    if constexpr (TILE) {
-        constexpr size_t lds = 2u * 16u * MT * 256u * XP;
-        auto* k = rows_tile_kernel<KIND, WP, XP, MT, FORM>;
-        hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), lds, s, a);
-    } else {
-        auto* k = rows_split_kernel<KIND, WP, XP, MT, FORM>;
-        hipLaunchKernelGGL(k, dim3((uint32_t)grid), dim3(256), 0, s, a, sh.kw);
-    }
-    return hipGetLastError();
+    return rows_launch(rows_tile_kernel<KIND, WP, XP, MT, FORM>, tiles, FORM == ROWS_GLU ? 8u : 16u, 256u, 2u * 16u * MT * 256u * XP, a, s);
+}
+
+template <int KIND, int WP, int XP, int MT, int FORM, int RT>
+hipError_t rows_go_split(const RowsShape& sh, RowsArgs a, hipStream_t s) {
+    const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles, sets = ROWS_SPLIT_WAVES / sh.kw;
+    return rows_launch(rows_split_kernel<KIND, WP, XP, MT, FORM, RT>, tiles, sets * (FORM == ROWS_GLU ? 1u : (uint32_t)RT),
+                       64u * ROWS_SPLIT_WAVES, (size_t)(ROWS_SPLIT_WAVES - sets) * MT * RT * 1024u, a, s, sh.kw);
 }
 
 template <int KIND, int WP, int XP, int FORM>
 hipError_t rows_mt(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
+    constexpr int RT = FORM == ROWS_LORA ? 1 : 2;
     if (sh.tile) {
-        if (sh.mt == 4) return rows_go<KIND, WP, XP, 4, FORM, true>(sh, a, s);
+        if (sh.mt == 4) return rows_go_tile<KIND, WP, XP, 4, FORM>(a, s);
         if constexpr (rows_tile8(KIND, WP, XP, FORM))
-            if (sh.mt == 8) return rows_go<KIND, WP, XP, 8, FORM, true>(sh, a, s);
+            if (sh.mt == 8) return rows_go_tile<KIND, WP, XP, 8, FORM>(a, s);
     } else {
-        if (sh.mt == 1) return rows_go<KIND, WP, XP, 1, FORM, false>(sh, a, s);
-        if (sh.mt == 4) return rows_go<KIND, WP, XP, 4, FORM, false>(sh, a, s);
+        if (sh.mt == 1) return rows_go_split<KIND, WP, XP, 1, FORM, RT>(sh, a, s);
+        if (sh.mt == 4) return rows_go_split<KIND, WP, XP, 4, FORM, RT>(sh, a, s);
     }
     return hipErrorInvalidValue;
 }
