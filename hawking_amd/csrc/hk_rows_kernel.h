@@ -141,19 +141,52 @@ __device__ __forceinline__ void rows_each(F&& f) {
 // for a slot that is not its own it counts as zero.  B comes RB slots at a time,
 // since a slot is one product and its latency is the cost.  T: the RT row tiles
 // of this wave; exps: this lane's position of every 16, updated.
+//
+// What the part needs first is read ahead (rows_lora_ahead), so a kernel can
+// ask for it before its own products.
+template <int MT>
+struct RowsLoraAhead {
+    uint32_t grouped, o0, o1, rank;  // of all slots; of slot lane
+    int32_t g[MT];
+    uint4 mid[MT];
+};
+__device__ __forceinline__ void rows_lora_slot(const RowsArgs& a, uint32_t s, uint32_t* o0, uint32_t* o1, uint32_t* rank) {
+    const RowsLora& L = a.lora;
+    const bool in = s < L.slots;
+    const uint32_t c = min(s, L.slots - 1u);
+    *o0 = min((uint32_t)max(ldg(L.offsets + c), 0), a.n);
+    *o1 = min((uint32_t)max(ldg(L.offsets + c + 1), 0), a.n);
+    *rank = ldg(&L.tab[c].rank);
+    if (!in) *o0 = *o1 = *rank = 0;
+}
+template <int MT>
+__device__ __forceinline__ void rows_lora_ahead(const RowsArgs& a, uint32_t first, uint32_t last, int lane, RowsLoraAhead<MT>& h) {
+    const RowsLora& L = a.lora;
+    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4, pitch = L.kk_max * 64u * L.planes;
+    h.grouped = min((uint32_t)max(ldg(L.offsets + L.slots), 0), a.n);
+    rows_lora_slot(a, (uint32_t)lane, &h.o0, &h.o1, &h.rank);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        // (rows without an adapter hold whatever the workspace held: not used)
+        const uint32_t p = min(first + 16u * mt + m, last - 1u);
+        h.g[mt] = ldg(L.mid_exps + p);
+        h.mid[mt] = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)p * pitch + 16u * q));
+    }
+}
 template <int MT, int RT>
 __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane,
-                                          uint32_t wk, uint32_t kw, int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
-    constexpr int RB = RT == 4 ? 2 : 8 / RT;
+                                          uint32_t wk, uint32_t kw, const RowsLoraAhead<MT>& h, int32_t* exps,
+                                          hk_f32x4 (&acc)[MT][RT]) {
+    constexpr int RB = RT == 4 ? 2 : 4;
     const RowsLora& L = a.lora;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
     const uint32_t pitch = L.kk_max * 64u * L.planes;
-    const uint32_t grouped = min((uint32_t)max(L.offsets[L.slots], 0), a.n);
+    const uint32_t grouped = __builtin_amdgcn_readfirstlane(h.grouped);
     if (first >= grouped) return;
     rows_each<MT>([&](auto mt) {
         const uint32_t p = first + 16u * mt + m;
         if (p < grouped) {
-            const int32_t g = L.mid_exps[p];
+            const int32_t g = h.g[mt];
             const bool nan = exps[mt] == ROWS_EXP_BAD || g == ROWS_EXP_BAD;
             const int d = nan ? 0 : g - exps[mt];
 #pragma unroll
@@ -171,17 +204,13 @@ __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uin
             uint4 mid[MT];
             rows_each<MT>([&](auto mt) {
                 const uint32_t p = min(f + 16u * mt + m, grouped - 1u);
-                mid[mt] = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)p * pitch + (pl * L.kk_max + k) * 64u + 16u * q));
+                if (k == 0 && pl == 0) mid[mt] = h.mid[mt];
+                else mid[mt] = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)p * pitch + (pl * L.kk_max + k) * 64u + 16u * q));
             });
             uint32_t seen = 0;  // slots of the tile so far
             for (uint32_t s0 = 0; s0 < L.slots; s0 += 64u) {
-                const uint32_t sl = s0 + (uint32_t)lane;
-                uint32_t o0 = 0, o1 = 0, rank = 0;
-                if (sl < L.slots) {
-                    o0 = min((uint32_t)max(L.offsets[sl], 0), a.n);
-                    o1 = min((uint32_t)max(L.offsets[sl + 1], 0), a.n);
-                    rank = L.tab[sl].rank;
-                }
+                uint32_t o0 = h.o0, o1 = h.o1, rank = h.rank;
+                if (s0) rows_lora_slot(a, s0 + (uint32_t)lane, &o0, &o1, &rank);
                 uint64_t hit = __ballot(o0 < last && o1 > first && o0 < o1 && rank > 32u * k);
                 while (hit) {
                     uint32_t s[RB], lo[RB], hi[RB];
@@ -189,7 +218,7 @@ __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uin
 #pragma unroll
                     for (int b = 0; b < RB; ++b) {
                         // this wave's next slot, if any
-                        while (hit && seen % kw != wk) {
+                        while (hit && (seen & (kw - 1u)) != wk) {  // (kw is a power of two)
                             hit &= hit - 1;
                             ++seen;
                         }
@@ -229,31 +258,6 @@ __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uin
                 }
             }
         }
-}
-
-// Scales a tile's sums back and stores them; GLU: row tiles r and r + RT / 2
-// are the gate and the up rows of the same outputs.
-template <int MT, int RT, bool GLU>
-__device__ __forceinline__ void rows_epilogue(const RowsArgs& a, uint32_t first, uint32_t last, uint32_t T0, int lane,
-                                              const int32_t* exps, hk_f32x4 (&acc)[MT][RT]) {
-    constexpr int RO = GLU ? RT / 2 : RT;
-    const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
-    float fin = 0.0f;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t p = first + 16u * mt + m;
-        uint32_t yr = p;
-        if (a.scatter && a.order && p < last) yr = (uint32_t)a.order[p];
-#pragma unroll
-        for (int r = 0; r < RO; ++r) {
-            const uint32_t row = 16u * (T0 + (uint32_t)r) + 4u * q;
-            float v[4];
-            rows_scale<GLU>(acc[mt][r], acc[mt][GLU ? r + RO : r], exps[mt], v, &fin);
-            // (a scattered row outside y was flagged when its source was looked up)
-            if (p < last && yr < a.n && row < a.rows) rows_store(a, yr, row, v);
-        }
-    }
-    if (__ballot(fin != fin) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
 }
 
 // ------------------------------------------------------------------ many rows a group: x through LDS
@@ -479,7 +483,11 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
     int32_t exps[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) exps[mt] = map[16 * mt + m].exp;
-    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, 0, 1, exps, acc);
+    if constexpr (FORM == ROWS_LORA) {
+        RowsLoraAhead<MT> ahead;
+        rows_lora_ahead<MT>(a, first, last, lane, ahead);
+        rows_lora<MT, RT>(a, first, last, T, lane, 0, 1, ahead, exps, acc);
+    }
     // (the last stage ended with a barrier: its buffers are free)
     rows_store_tile<MT, RT, GLU>(a, first, last, T0, lane, map, lds + wave * ROWS_OUT_BYTES, exps, acc);
 }
@@ -511,7 +519,7 @@ __global__ void __launch_bounds__(256, MT == 4 && WP == 1 && XP == 1 && KIND != 
 // (SwiGLU: one of the gate, one of the up organ); kw waves share a set, wave w
 // of them taking supersteps w, w + kw, ... and their sums are added in LDS in
 // wave order.  Such calls are bound by the weight stream and its latency: the
-// image is read straight from L2 (a product ahead, the weights a superstep
+// image is read straight from L2 (a stage ahead, the weights a superstep
 // ahead), without LDS or barriers in the loop.
 constexpr uint32_t ROWS_SPLIT_WAVES = 8;
 template <int KIND, int WP, int XP, int MT, int FORM, int RT>
@@ -519,9 +527,10 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
     constexpr int BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
     constexpr bool GLU = FORM == ROWS_GLU;
     extern __shared__ __align__(16) uint8_t lds[];
-    hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [8 - 8 / kw][MT * RT][64]
+    hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [waves][MT * RT][64]
+    __shared__ int32_t sexp[BM];
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave % kw, wr = wave / kw;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave & (kw - 1u), wr = wave / kw;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
 
     uint32_t tile, block, group, first, last;
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
         xs[mt] = a.ws.img + (size_t)src[mt] * pitch + 16u * q;
         any_bad |= bad[mt];
     }
-    hk_f16x8 x[2][MT][XP];
+    hk_f16x8 x[4][MT][XP];
     auto x_load = [&](uint32_t s, int u, hk_f16x8(&v)[MT][XP]) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -573,7 +582,10 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
                 v[mt][p] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
                                                             xs[mt] + (size_t)min(s, a.stages - 1u) * (256u * XP) + 256u * p + 64u * u)));
     };
-    x_load(wk * STG, 0, x[0]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x_load(wk * STG, u, x[u]);
+    RowsLoraAhead<MT> ahead;
+    if constexpr (FORM == ROWS_LORA) rows_lora_ahead<MT>(a, first, last, lane, ahead);
     // (read after the operands, so that they do not wait for it)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) exps[mt] = bad[mt] ? ROWS_EXP_BAD : a.ws.exps[src[mt]];
@@ -589,38 +601,54 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
         heads(t + 2u * kw);
         rows_each<STG * 4>([&](auto i) {
             constexpr int st = i / 4, u = i % 4;
-            // the next product's image: of this stage, the next one, or this wave's next superstep
-            x_load(u < 3 ? t * STG + st : st < STG - 1 ? t * STG + st + 1u : (t + kw) * STG, (u + 1) % 4, x[(u + 1) & 1]);
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 hk_f16x8 wh, wl;
                 rows_weights<KIND, WP>(cur[r], st, u, wh, wl);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[u & 1][mt], acc[mt][r]);
+                for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[u][mt], acc[mt][r]);
             }
+            // the same product of the next stage, or of this wave's next superstep
+            x_load(st < STG - 1 ? t * STG + st + 1u : (t + kw) * STG, u, x[u]);
         });
 #pragma unroll
         for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
     }
-    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, wk, kw, exps, acc);
-    if (kw > 1) {
-        // part[wave - wr - 1]: the waves that are not their set's first
-        if (wk) {
+    if constexpr (FORM == ROWS_LORA) rows_lora<MT, RT>(a, first, last, T, lane, wk, kw, ahead, exps, acc);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) part[((wave - wr - 1u) * (MT * RT) + mt * RT + r) * 64u + lane] = acc[mt][r];
-        }
-        __syncthreads();
-        if (wk) return;
-        for (uint32_t k = 1; k < kw; ++k)
+        for (int r = 0; r < RT; ++r) part[(wave * (MT * RT) + mt * RT + r) * 64u + lane] = acc[mt][r];
+    if (wave == 0 && q == 0) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) acc[mt][r] += part[((wave + k - wr - 1u) * (MT * RT) + mt * RT + r) * 64u + lane];
+        for (int mt = 0; mt < MT; ++mt) sexp[16 * mt + m] = exps[mt];
     }
-    if (T0 >= a.n_row_tiles) return;
-    rows_epilogue<MT, RT, GLU>(a, first, last, T0, lane, exps, acc);
+    __syncthreads();
+    // every thread sums, scales and stores whole lanes' results: one copy of
+    // that code, since a small call runs it once and its instructions' way to
+    // the CU is part of the call's time
+    constexpr uint32_t RO = GLU ? RT / 2 : RT, UNITS = MT * RO * 64u;
+    const uint32_t sets = ROWS_SPLIT_WAVES / kw;
+    float fin = 0.0f;
+    for (uint32_t i = threadIdx.x; i < sets * UNITS; i += 64u * ROWS_SPLIT_WAVES) {
+        const uint32_t set = i / UNITS, u = i % UNITS, l = u & 63u, r = (u >> 6) % RO, mt = (u >> 6) / RO;
+        const hk_f32x4* at = part + (set * kw * (MT * RT) + mt * RT + r) * 64u + l;
+        hk_f32x4 g = at[0], h = g;
+        if constexpr (GLU) h = at[RO * 64u];
+        for (uint32_t k = 1; k < kw; ++k) {
+            g += at[k * (MT * RT) * 64u];
+            if constexpr (GLU) h += at[(k * (MT * RT) + RO) * 64u];
+        }
+        const uint32_t tpos = 16u * mt + (l & 15u), p = first + tpos;
+        const uint32_t row = 16u * ((block * sets + set) * RO + r) + 4u * (l >> 4);
+        float v[4];
+        rows_scale<GLU>(g, h, sexp[tpos], v, &fin);
+        uint32_t yr = p;
+        if (a.scatter && a.order && p < last) yr = (uint32_t)a.order[p];
+        // (a scattered row outside y was flagged when its source was looked up)
+        if (p < last && yr < a.n && row < a.rows) rows_store(a, yr, row, v);
+    }
+    if (__ballot(fin != fin) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
 }
 
 // ------------------------------------------------------------------ one to four rows a group: the GEMV engine
@@ -855,7 +883,7 @@ template <int KIND, int WP, int XP, int MT, int FORM, int RT>
 hipError_t rows_go_split(const RowsShape& sh, RowsArgs a, hipStream_t s) {
     const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles, sets = ROWS_SPLIT_WAVES / sh.kw;
     return rows_launch(rows_split_kernel<KIND, WP, XP, MT, FORM, RT>, tiles, sets * (FORM == ROWS_GLU ? 1u : (uint32_t)RT),
-                       64u * ROWS_SPLIT_WAVES, (size_t)(ROWS_SPLIT_WAVES - sets) * MT * RT * 1024u, a, s, sh.kw);
+                       64u * ROWS_SPLIT_WAVES, (size_t)ROWS_SPLIT_WAVES * MT * RT * 1024u, a, s, sh.kw);
 }
 
 template <int KIND, int WP, int XP, int FORM>
