@@ -61,29 +61,35 @@ __global__ void __launch_bounds__(256) group_scan_kernel(const int32_t* __restri
 
 // ------------------------------------------------------------------ many ids: counts a part, then places
 
-constexpr uint32_t GROUP_WAVE_IDS = 256;  // ids of a wave
+constexpr int GROUP_ROUNDS = 4;                            // a wave's ids in rounds of 64
+constexpr uint32_t GROUP_WAVE_IDS = 64 * GROUP_ROUNDS;
+constexpr uint32_t GROUP_PARTS = 32;      // parts' counts in flight
 
-// part[b][key]: the ids of workgroup b's part with that key.
+// part[b][key]: the ids of workgroup b's part with that key, two 16-bit counts
+// a word (a part has at most 4096 ids).
 template <int NW>
 __global__ void __launch_bounds__(64 * NW) group_count_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t G,
                                                               uint32_t* __restrict__ part) {
-    extern __shared__ uint32_t cnt[];  // [G + 1]
-    for (uint32_t k = threadIdx.x; k <= G; k += 64u * NW) cnt[k] = 0;
+    extern __shared__ uint32_t cnt[];  // [words]
+    const uint32_t words = (G + 2u) / 2u;
+    for (uint32_t k = threadIdx.x; k < words; k += 64u * NW) cnt[k] = 0;
     __syncthreads();
     const uint32_t i0 = blockIdx.x * (NW * GROUP_WAVE_IDS);
-    int32_t v[4];
+    int32_t v[GROUP_ROUNDS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = ldg(ids + min(i0 + threadIdx.x + 64u * NW * (uint32_t)j, n - 1u));
+    for (int j = 0; j < GROUP_ROUNDS; ++j) v[j] = ldg(ids + min(i0 + threadIdx.x + 64u * NW * (uint32_t)j, n - 1u));
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (i0 + threadIdx.x + 64u * NW * (uint32_t)j < n) atomicAdd(&cnt[group_key(v[j], G)], 1u);
+    for (int j = 0; j < GROUP_ROUNDS; ++j) {
+        const uint32_t key = group_key(v[j], G);
+        if (i0 + threadIdx.x + 64u * NW * (uint32_t)j < n) atomicAdd(&cnt[key >> 1], 1u << (16u * (key & 1u)));
+    }
     __syncthreads();
-    for (uint32_t k = threadIdx.x; k <= G; k += 64u * NW) part[(size_t)blockIdx.x * (G + 1u) + k] = cnt[k];
+    for (uint32_t k = threadIdx.x; k < words; k += 64u * NW) part[(size_t)blockIdx.x * words + k] = cnt[k];
 }
 
 // Places.  The workgroup sums the counts of all parts (a key's offset is the
 // sum over smaller keys) and of the parts before its own; its waves count
-// their own 256 ids in LDS (16-bit counters, two a word), the counts of the
+// their own ids in LDS (16-bit counters, two a word), the counts of the
 // waves before give each wave its first place of a key, and the wave then
 // walks its ids 64 at a time: equal lanes find each other by one ballot a bit
 // of the key, and the lowest of them advances the counter.
@@ -96,33 +102,57 @@ __global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __r
     extern __shared__ uint32_t sm[];
     __shared__ uint32_t wsum[NW];
     const uint32_t keys = G + 1u, words = (keys + 1u) / 2u;
-    uint32_t* base = sm;               // [keys] first place of the key in this part
-    uint32_t* wcnt = sm + keys;        // [NW][words] 16-bit counters
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, b = blockIdx.x;
+    uint32_t* base = sm;         // [keys] ids of the key, then its first place in this part
+    uint32_t* wcnt = sm + keys;  // [NW][words] 16-bit counters
+    uint32_t* before = wcnt;     // [keys], until the counters are cleared: its ids in the parts before
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t b = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (b >= parts) return;
     uint32_t* mine = wcnt + wave * words;
-    for (uint32_t k = tid; k < NW * words; k += NT) wcnt[k] = 0;
+    for (uint32_t k = tid; k < 2u * keys; k += NT) sm[k] = 0;
 
     const uint32_t i0 = b * (NW * GROUP_WAVE_IDS) + wave * GROUP_WAVE_IDS;
-    uint32_t key[4];
+    uint32_t key[GROUP_ROUNDS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < GROUP_ROUNDS; ++j) {
         const uint32_t i = i0 + 64u * (uint32_t)j + lane;
         const int32_t v = ldg(ids + min(i, n - 1u));
         key[j] = i < n ? group_key(v, G) : 0xFFFFFFFFu;
     }
+    __syncthreads();
+    // the parts' counts: two keys a lane, the parts over as many slices of the
+    // waves as the keys leave waves for (a wave's parts are the same for all
+    // its lanes, so that their addresses are scalar work)
+    const uint32_t kw = (words + 63u) / 64u, slices = max((uint32_t)NW / kw, 1u);
+    const uint32_t slice = __builtin_amdgcn_readfirstlane(slices == 1 ? 0u : wave / kw);
+    if (slice < slices) {
+        for (uint32_t w = (slices == 1 ? wave : wave % kw) * 64u + lane; w < words; w += slices == 1 ? NT : words) {
+            uint32_t lo = 0, hi = 0, lo0 = 0, hi0 = 0;
+            for (uint32_t p0 = slice; p0 < parts; p0 += slices * GROUP_PARTS) {
+                uint32_t c[GROUP_PARTS];  // in flight together
+#pragma unroll
+                for (uint32_t j = 0; j < GROUP_PARTS; ++j) c[j] = ldg(part + (size_t)min(p0 + slices * j, parts - 1u) * words + w);
+#pragma unroll
+                for (uint32_t j = 0; j < GROUP_PARTS; ++j) {
+                    const uint32_t p = p0 + slices * j, v = p < parts ? c[j] : 0u, v0 = p < b ? c[j] : 0u;
+                    lo += v & 0xFFFFu, hi += v >> 16;
+                    lo0 += v0 & 0xFFFFu, hi0 += v0 >> 16;
+                }
+            }
+            atomicAdd(&base[2u * w], lo);
+            atomicAdd(&before[2u * w], lo0);
+            if (2u * w + 1u < keys) {
+                atomicAdd(&base[2u * w + 1u], hi);
+                atomicAdd(&before[2u * w + 1u], hi0);
+            }
+        }
+    }
+    __syncthreads();
     // this part's first place of every key: keys in runs of NT, a scan a run
     uint32_t run = 0;
     for (uint32_t k0 = 0; k0 < keys; k0 += NT) {
         const uint32_t k = k0 + tid;
-        uint32_t total = 0, before = 0;
-        if (k < keys) {
-#pragma unroll 8
-            for (uint32_t p = 0; p < parts; ++p) {
-                const uint32_t c = part[(size_t)p * keys + k];
-                total += c;
-                before += p < b ? c : 0u;
-            }
-        }
+        const uint32_t total = k < keys ? base[k] : 0u;
         const uint32_t inc = wave_incl_scan(total);
         __syncthreads();
         if (lane == 63u) wsum[wave] = inc;
@@ -134,18 +164,20 @@ __global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __r
         }
         off += inc - total;
         if (k < keys) {
-            base[k] = off + before;
+            base[k] = off + before[k];
             if (b == 0) offsets[k] = (int32_t)off;
         }
         run += all;
     }
-    // (the counters were cleared before the barriers above)
+    __syncthreads();
+    for (uint32_t k = tid; k < NW * words; k += NT) wcnt[k] = 0;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < GROUP_ROUNDS; ++j)
         if (key[j] != 0xFFFFFFFFu) atomicAdd(&mine[key[j] >> 1], 1u << (16u * (key[j] & 1u)));
     __syncthreads();
     for (uint32_t w = tid; w < words; w += NT) {
-        uint32_t sum = 0;  // at most NW * 256 ids a part: no carry between the halves
+        uint32_t sum = 0;  // at most NW * GROUP_WAVE_IDS ids a part: no carry between the halves
 #pragma unroll
         for (uint32_t v = 0; v < (uint32_t)NW; ++v) {
             const uint32_t c = wcnt[v * words + w];
@@ -155,7 +187,7 @@ __global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __r
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < GROUP_ROUNDS; ++j) {
         const bool in = key[j] != 0xFFFFFFFFu;
         uint64_t same = __ballot(in);
         for (uint32_t t = 0; t < bits; ++t) {
@@ -186,7 +218,7 @@ static uint32_t group_part_ids(uint32_t G) { return (G <= 2048u ? 16u : 4u) * GR
 
 size_t group_rows_ws_bytes(uint32_t n, uint32_t G) {
     if (n == 0 || group_scans(n, G)) return 0;
-    return (size_t)((n + group_part_ids(G) - 1u) / group_part_ids(G)) * (G + 1u) * 4u;
+    return (size_t)((n + group_part_ids(G) - 1u) / group_part_ids(G)) * ((G + 2u) / 2u) * 4u;
 }
 
 template <int NW>
@@ -196,8 +228,8 @@ static hipError_t group_parts(const int32_t* ids, uint32_t n, uint32_t G, int32_
     uint32_t bits = 0;
     while ((G >> bits) != 0) ++bits;
     const size_t lds = ((size_t)keys + (size_t)NW * ((keys + 1u) / 2u)) * 4u;
-    hipLaunchKernelGGL(group_count_kernel<NW>, dim3(parts), dim3(64 * NW), keys * 4u, s, ids, n, G, part);
-    hipLaunchKernelGGL(group_place_kernel<NW>, dim3(parts), dim3(64 * NW), lds, s, ids, n, G, bits, part, parts, offsets,
+    hipLaunchKernelGGL(group_count_kernel<NW>, dim3(parts), dim3(64 * NW), (keys + 1u) / 2u * 4u, s, ids, n, G, part);
+    hipLaunchKernelGGL(group_place_kernel<NW>, dim3((parts + 7u) / 8u * 8u), dim3(64 * NW), lds, s, ids, n, G, bits, part, parts, offsets,
                        order, pos);
     return hipGetLastError();
 }

@@ -102,74 +102,109 @@ hipError_t launch_lora_pack(const void* a, const void* b, int type, uint32_t ran
 
 // ------------------------------------------------------------------ A x
 
-// A workgroup: 16 positions of one slot, all RT rank tiles, the stages of the
+// A workgroup: 16 MT positions of one slot, all RT rank tiles, the stages of the
 // image split over NW waves (wave w takes stages w, w + NW, ...) and summed
-// in wave order.  The first wave then holds whole mid rows: a row is scaled
+// in wave order.  A wave then holds whole mid rows: a row is scaled
 // by the power of two that brings its maximum into [2^13, 2^14) and stored as
 // f16 (planes = 2: with the rounding error as a second f16).  mid_exps is the
 // exponent of y's part: B mid = sums * 2^-mid_exps, kept at most 80 above the
 // row's own exponent so that W x fits f32 in those units.
-template <int XP, int RT, int NW>
+template <int XP, int RT, int NW, int MT>
 __global__ void __launch_bounds__(64 * NW) lora_shrink_kernel(RowsArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [NW - 1][RT][64]
+    hk_f32x4* part = reinterpret_cast<hk_f32x4*>(lds);  // [NW - 1][MT][RT][64]
     const int lane = threadIdx.x & 63;
     const uint32_t wave = threadIdx.x >> 6, m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
-    const RowsTile tile = a.ws.tiles[blockIdx.x];
+    // consecutive tiles, which share a slot, to one XCD's L2 (workgroups go round the XCDs)
+    const uint32_t at = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= a.ws.max_tiles) return;
+    const RowsTile tile = a.ws.tiles[at];
     if (tile.first >= tile.last) return;
-    const uint32_t p = min(tile.first + m, tile.last - 1u);
     const LoraSlot slot = a.lora.tab[tile.group];
     const uint32_t rt_used = min((slot.rank + 15u) / 16u, (uint32_t)RT);
-    uint32_t r = p;
-    if (a.order) r = (uint32_t)a.order[p] / a.per_row;
-    const bool bad = r >= a.n_src;
-    if (bad) r = 0;
-    const uint8_t* x = a.ws.img + (size_t)r * a.stages * (256u * XP) + 16u * q;
+    uint32_t r[MT];
+    bool bad[MT];
+    const uint8_t* x[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        r[mt] = min(tile.first + 16u * mt + m, tile.last - 1u);
+        if (a.order) r[mt] = (uint32_t)a.order[r[mt]] / a.per_row;
+        bad[mt] = r[mt] >= a.n_src;
+        if (bad[mt]) r[mt] = 0;
+        x[mt] = a.ws.img + (size_t)r[mt] * a.stages * (256u * XP) + 16u * q;
+    }
     const uint8_t* w = a.lora.a + (size_t)tile.group * (2u * a.lora.kk_max) * a.stages * 4096u + 16u * (uint32_t)lane;
-    hk_f32x4 acc[RT];
+    hk_f32x4 acc[MT][RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) acc[i] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[mt][i] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
     for (uint32_t s = wave; s < a.stages; s += NW) {
-        hk_f16x8 xv[4][XP];
+        hk_f16x8 xv[MT][4][XP];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int pl = 0; pl < XP; ++pl)
-                xv[u][pl] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(x + (size_t)s * (256u * XP) + 256u * pl + 64u * u)));
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            if ((uint32_t)i < rt_used) {
+                for (int pl = 0; pl < XP; ++pl)
+                    xv[mt][u][pl] = __builtin_bit_cast(
+                        hk_f16x8, ldg(reinterpret_cast<const uint4*>(x[mt] + (size_t)s * (256u * XP) + 256u * pl + 64u * u)));
+        // four rank tiles' loads go out together: one at a time, the wave
+        // would wait for memory once a tile
+        constexpr int C = RT < 4 ? RT : 4;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const hk_f16x8 wv = __builtin_bit_cast(
-                        hk_f16x8, ldg(reinterpret_cast<const uint4*>(w + ((size_t)i * a.stages + s) * 4096u + 1024u * u)));
-                    acc[i] = rows_mfma<1, XP>(wv, wv, xv[u], acc[i]);
+        for (int i0 = 0; i0 < RT; i0 += C) {
+            hk_f16x8 wv[C][4];
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if ((uint32_t)(i0 + i) < rt_used) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        wv[i][u] = __builtin_bit_cast(
+                            hk_f16x8, ldg(reinterpret_cast<const uint4*>(w + ((size_t)(i0 + i) * a.stages + s) * 4096u + 1024u * u)));
                 }
-            }
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if ((uint32_t)(i0 + i) < rt_used) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+                            acc[mt][i0 + i] = rows_mfma<1, XP>(wv[i][u], wv[i][u], xv[mt][u], acc[mt][i0 + i]);
+                }
         }
     }
-    if (wave) {
+    // wave mt sums and stores positions 16 mt ... 16 mt + 15
 #pragma unroll
-        for (int i = 0; i < RT; ++i) part[((wave - 1u) * RT + i) * 64u + lane] = acc[i];
-    }
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) part[((wave * MT + mt) * RT + i) * 64u + lane] = acc[mt][i];
     __syncthreads();
-    if (wave) return;
+    if (wave >= MT) return;
+    const uint32_t pos = 16u * wave + m, p = min(tile.first + pos, tile.last - 1u);
+    uint32_t src = r[0];
+    bool out_of = bad[0];
+#pragma unroll
+    for (int mt = 1; mt < MT; ++mt)
+        if (wave == (uint32_t)mt) src = r[mt], out_of = bad[mt];
+    hk_f32x4 sum[RT];
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-        for (uint32_t k = 0; k + 1u < (uint32_t)NW; ++k) acc[i] += part[(k * RT + i) * 64u + lane];
+        sum[i] = part[(wave * RT + i) * 64u + lane];
+        for (uint32_t k = 1; k < (uint32_t)NW; ++k) sum[i] += part[((k * MT + wave) * RT + i) * 64u + lane];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            acc[i][j] *= slot.scale;
-            top = fmaxf(top, fabsf(acc[i][j]));
+            sum[i][j] *= slot.scale;
+            top = fmaxf(top, fabsf(sum[i][j]));
         }
     }
     // the row's four lanes
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    if (tile.first + m >= tile.last) return;
-    const int32_t E = a.ws.exps[r];
-    const bool nan = bad || E == ROWS_EXP_BAD || slot.a_exp == ROWS_EXP_BAD || slot.b_exp == ROWS_EXP_BAD || !isfinite(top);
+    if (tile.first + pos >= tile.last) return;
+    const int32_t E = a.ws.exps[src];
+    const bool nan = out_of || E == ROWS_EXP_BAD || slot.a_exp == ROWS_EXP_BAD || slot.b_exp == ROWS_EXP_BAD || !isfinite(top);
     int g = 0, out = 0;
     if (!nan) {
         out = E;
@@ -186,7 +221,7 @@ __global__ void __launch_bounds__(64 * NW) lora_shrink_kernel(RowsArgs a) {
     }
     if (q == 0) {
         a.lora.mid_exps[p] = nan ? ROWS_EXP_BAD : out;
-        if (bad) atomicOr(a.status, ROWS_ERR_ROUTE);
+        if (out_of) atomicOr(a.status, ROWS_ERR_ROUTE);
     }
     uint8_t* o = a.lora.mid + (size_t)p * a.lora.planes * a.lora.kk_max * 64u;
 #pragma unroll
@@ -195,34 +230,43 @@ __global__ void __launch_bounds__(64 * NW) lora_shrink_kernel(RowsArgs a) {
         uint16_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float v = nan ? 0.0f : ldexpf(acc[i][j], g);
+            const float v = nan ? 0.0f : ldexpf(sum[i][j], g);
             h[j] = f32_to_f16_bits(v);
             l[j] = f32_to_f16_bits(v - f16_bits_to_f32(h[j]));
         }
-        uint8_t* at = o + 32u * i + 8u * q;
-        *reinterpret_cast<uint2*>(at) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+        uint8_t* to = o + 32u * i + 8u * q;
+        *reinterpret_cast<uint2*>(to) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
         if (a.lora.planes == 2)
-            *reinterpret_cast<uint2*>(at + a.lora.kk_max * 64u) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
+            *reinterpret_cast<uint2*>(to + a.lora.kk_max * 64u) = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
     }
 }
 
-template <int XP, int RT, int NW>
+template <int XP, int RT, int NW, int MT>
 static hipError_t shrink_go(const RowsArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((lora_shrink_kernel<XP, RT, NW>), dim3(a.ws.max_tiles), dim3(64 * NW), (size_t)(NW - 1) * RT * 1024u, s, a);
+    hipLaunchKernelGGL((lora_shrink_kernel<XP, RT, NW, MT>), dim3((a.ws.max_tiles + 7u) / 8u * 8u), dim3(64 * NW),
+                       (size_t)NW * MT * RT * 1024u, s, a);
     return hipGetLastError();
 }
 
-template <int XP>
-static hipError_t shrink_rank(const RowsArgs& a, hipStream_t s) {
-    const uint32_t tiles = 2u * a.lora.kk_max;
-    if (tiles <= 2) return shrink_go<XP, 2, 8>(a, s);
-    if (tiles <= 4) return shrink_go<XP, 4, 8>(a, s);
-    if (tiles <= 8) return shrink_go<XP, 8, 4>(a, s);
-    return shrink_go<XP, 16, 4>(a, s);
+uint32_t lora_shrink_rows(uint32_t n, uint32_t slots, uint32_t kk_max) {
+    return kk_max <= 2 && n / std::max(1u, std::min(n, slots)) >= 64 ? 32 : 16;
 }
 
-hipError_t launch_lora_shrink(const RowsArgs& a, int xp, hipStream_t s) {
-    return xp == 2 ? shrink_rank<2>(a, s) : shrink_rank<1>(a, s);
+template <int XP, int MT>
+static hipError_t shrink_rank(const RowsArgs& a, hipStream_t s) {
+    const uint32_t tiles = 2u * a.lora.kk_max;
+    if (tiles <= 2) return shrink_go<XP, 2, 8, MT>(a, s);
+    if constexpr (MT == 2) return shrink_go<XP, 4, 8, 2>(a, s);
+    else {
+        if (tiles <= 4) return shrink_go<XP, 4, 8, 1>(a, s);
+        if (tiles <= 8) return shrink_go<XP, 8, 4, 1>(a, s);
+        return shrink_go<XP, 16, 4, 1>(a, s);
+    }
+}
+
+hipError_t launch_lora_shrink(const RowsArgs& a, int xp, uint32_t rows, hipStream_t s) {
+    if (rows == 32) return xp == 2 ? shrink_rank<2, 2>(a, s) : shrink_rank<1, 2>(a, s);
+    return xp == 2 ? shrink_rank<2, 1>(a, s) : shrink_rank<1, 1>(a, s);
 }
 
 }  // namespace hk

@@ -280,7 +280,9 @@ hipError_t launch_rows_image(const void* x, int x_type, size_t x_stride, uint32_
                              const RowsWs& ws, const int32_t* offsets, uint32_t groups, uint32_t n_pos, uint32_t tile_rows,
                              uint32_t* status, hipStream_t s);
 // The adapters' first half, A_s x of every position with an adapter, into lora.mid.
-hipError_t launch_lora_shrink(const RowsArgs& a, int xp, hipStream_t s);
+// the rows a workgroup of the adapters' first half takes (the tile list is made for them)
+uint32_t lora_shrink_rows(uint32_t n, uint32_t slots, uint32_t kk_max);
+hipError_t launch_lora_shrink(const RowsArgs& a, int xp, uint32_t rows, hipStream_t s);
 // An adapter into slot `slot`; a [rank x cols], b [rows x rank] of `type` (device).
 hipError_t launch_lora_pack(const void* a, const void* b, int type, uint32_t rank, uint32_t rows, uint32_t cols, int kind,
                             float scale, uint32_t slot, uint32_t kk_max, LoraSlot* tab, uint8_t* a_bank, uint8_t* b_bank,

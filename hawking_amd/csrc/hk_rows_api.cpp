@@ -301,8 +301,9 @@ extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_ba
     const RowsShape sh = shape_for(f.kind, ROWS_LORA, x->type, y->type, y->n, 1, x->n, f.cols, f.n_tiles);
     RowsArgs a{};
     a.organs = static_cast<const OrganView*>(organ->view_dev);
-    // the adapters' first half works on tiles of 16 rows of one slot
-    a.ws = ws_views(ws, L, max_tiles(y->n, bank->n_slots, 16));
+    // the adapters' first half works on tiles of rows of one slot
+    const uint32_t tile_rows = lora_shrink_rows(y->n, bank->n_slots, bank->kk_max);
+    a.ws = ws_views(ws, L, max_tiles(y->n, bank->n_slots, tile_rows));
     a.order = order;
     a.per_row = 1;
     a.n = y->n;
@@ -319,9 +320,9 @@ extern "C" int hk_gemm_lora(hk_ctx* ctx, const hk_organ* organ, const hk_lora_ba
     a.lora = {offsets, bank->tab, bank->a, bank->b, b + L.mid, reinterpret_cast<int32_t*>(b + L.mid_exps),
               bank->n_slots, bank->kk_max, (uint32_t)mid_planes};
     int rc = check_hip(ctx, launch_rows_image(x->data, x->type, x->stride, x->n, f.cols, f.kind, sh.xp, a.ws, offsets,
-                                              bank->n_slots, y->n, 16, ctx->dev_status, st),
+                                              bank->n_slots, y->n, tile_rows, ctx->dev_status, st),
                        "row image launch");
-    if (!rc) rc = check_hip(ctx, launch_lora_shrink(a, sh.xp, st), "adapter launch");
+    if (!rc) rc = check_hip(ctx, launch_lora_shrink(a, sh.xp, tile_rows, st), "adapter launch");
     if (!rc) rc = check_hip(ctx, launch_rows_product(sh, a, st), "row product launch");
     return rc;
 }
