@@ -105,6 +105,19 @@ def test_ranks(ctx, oracle, max_rank, ranks, x_type, y_type, a_type):
         _run(ctx, oracle, "q4", 80, 256, _mix(np.random.default_rng(n), n, len(ranks)), ranks, max_rank, x_type, y_type, a_type)
 
 
+@pytest.mark.parametrize("x_type,y_type", TYPES)
+@pytest.mark.parametrize("ranks,max_rank", [([16, 9], 16), ([64, 33, 5, 0], 64), ([128, 40], 128)])
+def test_many_rows_a_slot(ctx, oracle, ranks, max_rank, x_type, y_type):
+    """Slots of hundreds of rows, and one of a single row among them."""
+    say("lora many rows", ranks, x_type, y_type)
+    rng = np.random.default_rng(len(ranks))
+    for n in (64 * len(ranks) - 1, 64 * len(ranks), 531):
+        ids = _mix(rng, n, len(ranks))
+        ids[ids == len(ranks) - 1] = 0
+        ids[n // 2] = len(ranks) - 1
+        _run(ctx, oracle, "q4", 52, 288, ids, ranks, max_rank, x_type, y_type)
+
+
 @pytest.mark.parametrize("ids", [[-1] * 20, [0] * 150, [2] * 5 + [-1] * 5, list(range(70)), [9999, -7, 1]])
 def test_who_has_an_adapter(ctx, oracle, ids):
     """No row, every row, one slot of many, a slot a row (one tile, many adapters)."""
