@@ -597,8 +597,9 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[mt][r] = hk_f32x4{0.f, 0.f, 0.f, 0.f};
     for (uint32_t t = wk; t < n_super; t += kw) {
-        w_load(t + kw, nxt);
-        heads(t + 2u * kw);
+        const bool more = t + kw < n_super;  // (what is in flight at the end, the waves would wait for)
+        if (more) w_load(t + kw, nxt);
+        if (more) heads(t + 2u * kw);
         rows_each<STG * 4>([&](auto i) {
             constexpr int st = i / 4, u = i % 4;
 #pragma unroll
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
                 for (int mt = 0; mt < MT; ++mt) acc[mt][r] = rows_mfma<WP, XP>(wh, wl, x[u][mt], acc[mt][r]);
             }
             // the same product of the next stage, or of this wave's next superstep
-            x_load(st < STG - 1 ? t * STG + st + 1u : (t + kw) * STG, u, x[u]);
+            if (st < STG - 1 || more) x_load(st < STG - 1 ? t * STG + st + 1u : (t + kw) * STG, u, x[u]);
         });
 #pragma unroll
         for (int r = 0; r < RT; ++r) cur[r] = nxt[r];
