@@ -558,18 +558,27 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
         for (int r = 0; r < RT; ++r) rows_fetch<KIND>(view(r), T[r], min(t, n_super - 1u), lane, hdr[r], w[r]);
     };
     heads(wk);
+    // (asked for before the weights: loads arrive in order, and the image's
+    // addresses would wait for the weights)
+    uint32_t src[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        src[mt] = min(first + 16u * mt + m, last - 1u);
+        if (a.order) src[mt] = (uint32_t)ldg(a.order + src[mt]);
+    }
+    asm volatile("" ::: "memory");
     w_load(wk, cur);
     heads(wk + kw);
 
     const size_t pitch = (size_t)a.stages * 256u * XP;
     const uint8_t* xs[MT];
     int32_t exps[MT];
-    uint32_t src[MT];
     bool bad[MT], any_bad = false;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) src[mt] = rows_source(a, min(first + 16u * mt + m, last - 1u), &bad[mt]);
-#pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
+        if (a.per_row != 1u) src[mt] /= a.per_row;
+        bad[mt] = src[mt] >= a.n_src;
+        if (bad[mt]) src[mt] = 0;
         xs[mt] = a.ws.img + (size_t)src[mt] * pitch + 16u * q;
         any_bad |= bad[mt];
     }
