@@ -142,14 +142,9 @@ __device__ __forceinline__ void rows_each(F&& f) {
 // since a slot is one product and its latency is the cost.  T: the RT row tiles
 // of this wave; exps: this lane's position of every 16, updated.
 //
-// What the part needs first is read ahead (rows_lora_ahead), so a kernel can
-// ask for it before its own products.
-template <int MT>
-struct RowsLoraAhead {
-    uint32_t grouped, o0, o1, rank;  // of all slots; of slot lane
-    int32_t g[MT];
-    uint4 mid[MT];
-};
+// What the part needs first is read ahead, so a kernel can ask for it before
+// its own products: rows_lora_slot the slots' positions, rows_lora_ahead the
+// mid rows and the first RB slots' B.
 __device__ __forceinline__ void rows_lora_slot(const RowsArgs& a, uint32_t s, uint32_t* o0, uint32_t* o1, uint32_t* rank) {
     const RowsLora& L = a.lora;
     const bool in = s < L.slots;
@@ -159,12 +154,62 @@ __device__ __forceinline__ void rows_lora_slot(const RowsArgs& a, uint32_t s, ui
     *rank = ldg(&L.tab[c].rank);
     if (!in) *o0 = *o1 = *rank = 0;
 }
-template <int MT>
-__device__ __forceinline__ void rows_lora_ahead(const RowsArgs& a, uint32_t first, uint32_t last, int lane, RowsLoraAhead<MT>& h) {
+template <int RT>
+struct RowsLoraPick {
+    static constexpr int RB = RT == 4 ? 2 : 4;
+    uint32_t s[RB], lo[RB], hi[RB];
+    int n;
+    hk_f16x8 w[RB][RT];
+
+    // This wave's next slots among those of hit, slots s0 + bit, and part k of their B.
+    __device__ __forceinline__ void next(const RowsArgs& a, const uint32_t* T, uint32_t k, uint32_t s0, uint32_t o0, uint32_t o1,
+                                         uint64_t* hit, uint32_t* seen, uint32_t wk, uint32_t kw, int lane) {
+        n = 0;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            while (*hit && (*seen & (kw - 1u)) != wk) {  // (kw is a power of two)
+                *hit &= *hit - 1;
+                ++*seen;
+            }
+            s[b] = s0, lo[b] = hi[b] = 0;
+            if (*hit) {
+                const int i = __builtin_ctzll(*hit);
+                *hit &= *hit - 1;
+                ++*seen;
+                s[b] = s0 + (uint32_t)i;
+                lo[b] = __builtin_amdgcn_readlane(o0, i);
+                hi[b] = __builtin_amdgcn_readlane(o1, i);
+                n = b + 1;
+            }
+        }
+        if (n == 0) return;
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                w[b][r] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
+                    a.lora.b + (((size_t)s[b] * a.n_row_tiles + T[r]) * a.lora.kk_max + k) * 1024u + 16u * (uint32_t)lane)));
+    }
+};
+template <int MT, int RT>
+struct RowsLoraAhead {
+    uint32_t grouped, o0, o1, rank;  // of all slots; of slot lane
+    int32_t g[MT];
+    uint4 mid[MT];
+    RowsLoraPick<RT> pick;
+    uint64_t hit;   // slots left of the first 64, after pick
+    uint32_t seen;  // slots of the tile so far
+};
+template <int MT, int RT>
+__device__ __forceinline__ void rows_lora_offsets(const RowsArgs& a, int lane, RowsLoraAhead<MT, RT>& h) {
+    h.grouped = min((uint32_t)max(ldg(a.lora.offsets + a.lora.slots), 0), a.n);
+    rows_lora_slot(a, (uint32_t)lane, &h.o0, &h.o1, &h.rank);
+}
+template <int MT, int RT>
+__device__ __forceinline__ void rows_lora_ahead(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane,
+                                                uint32_t wk, uint32_t kw, RowsLoraAhead<MT, RT>& h) {
     const RowsLora& L = a.lora;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4, pitch = L.kk_max * 64u * L.planes;
-    h.grouped = min((uint32_t)max(ldg(L.offsets + L.slots), 0), a.n);
-    rows_lora_slot(a, (uint32_t)lane, &h.o0, &h.o1, &h.rank);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         // (rows without an adapter hold whatever the workspace held: not used)
@@ -172,12 +217,14 @@ __device__ __forceinline__ void rows_lora_ahead(const RowsArgs& a, uint32_t firs
         h.g[mt] = ldg(L.mid_exps + p);
         h.mid[mt] = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)p * pitch + 16u * q));
     }
+    h.hit = __ballot(h.o0 < last && h.o1 > first && h.o0 < h.o1 && h.rank > 0u);
+    h.seen = 0;
+    h.pick.next(a, T, 0, 0, h.o0, h.o1, &h.hit, &h.seen, wk, kw, lane);
 }
 template <int MT, int RT>
 __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uint32_t last, const uint32_t* T, int lane,
-                                          uint32_t wk, uint32_t kw, const RowsLoraAhead<MT>& h, int32_t* exps,
+                                          uint32_t wk, uint32_t kw, RowsLoraAhead<MT, RT>& h, int32_t* exps,
                                           hk_f32x4 (&acc)[MT][RT]) {
-    constexpr int RB = RT == 4 ? 2 : 4;
     const RowsLora& L = a.lora;
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
     const uint32_t pitch = L.kk_max * 64u * L.planes;
@@ -196,6 +243,8 @@ __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uin
             exps[mt] = nan ? ROWS_EXP_BAD : g;
         }
     });
+    RowsLoraPick<RT>& pick = h.pick;
+    bool ready = true;  // pick holds the next slots
     for (uint32_t k = 0; k < L.kk_max; ++k)
         for (uint32_t pl = 0; pl < L.planes; ++pl) {
             // opaque to the compiler: it would keep the MT rows' addresses in registers over the loops, and spill
@@ -207,51 +256,27 @@ __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uin
                 if (k == 0 && pl == 0) mid[mt] = h.mid[mt];
                 else mid[mt] = ldg(reinterpret_cast<const uint4*>(L.mid + (size_t)p * pitch + (pl * L.kk_max + k) * 64u + 16u * q));
             });
-            uint32_t seen = 0;  // slots of the tile so far
+            uint32_t seen = ready ? h.seen : 0u;
             for (uint32_t s0 = 0; s0 < L.slots; s0 += 64u) {
                 uint32_t o0 = h.o0, o1 = h.o1, rank = h.rank;
                 if (s0) rows_lora_slot(a, s0 + (uint32_t)lane, &o0, &o1, &rank);
-                uint64_t hit = __ballot(o0 < last && o1 > first && o0 < o1 && rank > 32u * k);
-                while (hit) {
-                    uint32_t s[RB], lo[RB], hi[RB];
-                    int n = 0;
+                uint64_t hit = ready ? h.hit : __ballot(o0 < last && o1 > first && o0 < o1 && rank > 32u * k);
+                for (;;) {
+                    if (!ready) pick.next(a, T, k, s0, o0, o1, &hit, &seen, wk, kw, lane);
+                    ready = false;
+                    if (pick.n == 0) break;
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        // this wave's next slot, if any
-                        while (hit && (seen & (kw - 1u)) != wk) {  // (kw is a power of two)
-                            hit &= hit - 1;
-                            ++seen;
-                        }
-                        s[b] = s0, lo[b] = hi[b] = 0;
-                        if (hit) {
-                            const int i = __builtin_ctzll(hit);
-                            hit &= hit - 1;
-                            ++seen;
-                            s[b] = s0 + (uint32_t)i;
-                            lo[b] = __builtin_amdgcn_readlane(o0, i);
-                            hi[b] = __builtin_amdgcn_readlane(o1, i);
-                            n = b + 1;
-                        }
-                    }
-                    hk_f16x8 w[RB][RT];
-#pragma unroll
-                    for (int b = 0; b < RB; ++b)
-#pragma unroll
-                        for (int r = 0; r < RT; ++r)
-                            w[b][r] = __builtin_bit_cast(hk_f16x8, ldg(reinterpret_cast<const uint4*>(
-                                L.b + (((size_t)s[b] * a.n_row_tiles + T[r]) * L.kk_max + k) * 1024u + 16u * (uint32_t)lane)));
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        if (b >= n) break;
+                    for (int b = 0; b < pick.RB; ++b) {
+                        if (b >= pick.n) break;
                         rows_each<MT>([&](auto mt) {
                             const uint32_t t0 = f + 16u * mt, p = t0 + m;
-                            if (t0 < hi[b] && t0 + 16u > lo[b]) {  // uniform
-                                const bool mine = p >= lo[b] && p < hi[b];
+                            if (t0 < pick.hi[b] && t0 + 16u > pick.lo[b]) {  // uniform
+                                const bool mine = p >= pick.lo[b] && p < pick.hi[b];
                                 const uint4 v = mid[mt];
                                 const hk_f16x8 x = __builtin_bit_cast(
                                     hk_f16x8, make_uint4(mine ? v.x : 0u, mine ? v.y : 0u, mine ? v.z : 0u, mine ? v.w : 0u));
 #pragma unroll
-                                for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(w[b][r], x, acc[mt][r]);
+                                for (int r = 0; r < RT; ++r) acc[mt][r] = mfma_f16(pick.w[b][r], x, acc[mt][r]);
                             }
                         });
                     }
@@ -484,8 +509,9 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) exps[mt] = map[16 * mt + m].exp;
     if constexpr (FORM == ROWS_LORA) {
-        RowsLoraAhead<MT> ahead;
-        rows_lora_ahead<MT>(a, first, last, lane, ahead);
+        RowsLoraAhead<MT, RT> ahead;
+        rows_lora_offsets(a, lane, ahead);
+        rows_lora_ahead(a, first, last, T, lane, 0, 1, ahead);
         rows_lora<MT, RT>(a, first, last, T, lane, 0, 1, ahead, exps, acc);
     }
     // (the last stage ended with a barrier: its buffers are free)
@@ -566,6 +592,8 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
         src[mt] = min(first + 16u * mt + m, last - 1u);
         if (a.order) src[mt] = (uint32_t)ldg(a.order + src[mt]);
     }
+    RowsLoraAhead<MT, RT> ahead;
+    if constexpr (FORM == ROWS_LORA) rows_lora_offsets(a, lane, ahead);
     asm volatile("" ::: "memory");
     w_load(wk, cur);
     heads(wk + kw);
@@ -593,8 +621,7 @@ __global__ void __launch_bounds__(64 * ROWS_SPLIT_WAVES) rows_split_kernel(RowsA
     };
 #pragma unroll
     for (int u = 0; u < 4; ++u) x_load(wk * STG, u, x[u]);
-    RowsLoraAhead<MT> ahead;
-    if constexpr (FORM == ROWS_LORA) rows_lora_ahead<MT>(a, first, last, lane, ahead);
+    if constexpr (FORM == ROWS_LORA) rows_lora_ahead(a, first, last, T, lane, wk, kw, ahead);
     // (read after the operands, so that they do not wait for it)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) exps[mt] = bad[mt] ? ROWS_EXP_BAD : a.ws.exps[src[mt]];
