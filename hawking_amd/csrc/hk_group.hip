@@ -6,7 +6,8 @@
 // key, an id's place = offsets[key] + earlier ids of the same key.  Places
 // come from counts in a fixed order, never from the order atomics arrive in.
 // It reads 4 n bytes and writes 8 n + 4 (n_groups + 1): for every n that a
-// batch has the bound is latency (a launch, two dependent passes over ids).
+// batch has the bound is latency (512 ids of 256 groups 4.3 us, a launch that
+// does nothing 3.6; 327,680 ids of 512 groups 12.9, two launches).
 #include "hk_rows.h"
 
 namespace hk {
@@ -209,15 +210,16 @@ __global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __r
     }
 }
 
-// The one-launch form reads all ids in every workgroup, 256 threads of it.
-constexpr uint64_t GROUP_SCAN_READS = 1ull << 22;
+// The one-launch form reads all ids in every workgroup, so its time goes with
+// the ids where the other's hardly does.  Both in us for 4096 / 8192 / 16384
+// ids: 64 groups 6.7 / 10.3 / 18.4 and 10.0 / 10.3 / 10.3, 512 groups 6.5 /
+// 10.8 / 19.5 and 10.7 / 11.3 / 11.9, 8192 groups 16 / 32 / 66 and 41 / 42 / 42.
 constexpr uint32_t GROUP_SCAN_IDS = 8192;
 
-static bool group_scans(uint32_t n, uint32_t G) { return n <= GROUP_SCAN_IDS && (uint64_t)n * (G + 1u) <= GROUP_SCAN_READS; }
 static uint32_t group_part_ids(uint32_t G) { return (G <= 2048u ? 16u : 4u) * GROUP_WAVE_IDS; }
 
 size_t group_rows_ws_bytes(uint32_t n, uint32_t G) {
-    if (n == 0 || group_scans(n, G)) return 0;
+    if (n <= GROUP_SCAN_IDS) return 0;
     return (size_t)((n + group_part_ids(G) - 1u) / group_part_ids(G)) * ((G + 2u) / 2u) * 4u;
 }
 
@@ -236,7 +238,7 @@ static hipError_t group_parts(const int32_t* ids, uint32_t n, uint32_t G, int32_
 
 hipError_t launch_group_rows(const int32_t* ids, uint32_t n, uint32_t G, int32_t* offsets, int32_t* order, int32_t* pos,
                              void* ws, hipStream_t s) {
-    if (group_scans(n, G)) {
+    if (n <= GROUP_SCAN_IDS) {
         hipLaunchKernelGGL(group_scan_kernel, dim3(G + 1u), dim3(256), 0, s, ids, n, G, offsets, order, pos);
         return hipGetLastError();
     }

@@ -248,8 +248,9 @@ static hipError_t shrink_go(const RowsArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+constexpr uint32_t SHRINK_WIDE_ROWS = 4096;
 uint32_t lora_shrink_rows(uint32_t n, uint32_t slots, uint32_t kk_max) {
-    return kk_max <= 2 && n / std::max(1u, std::min(n, slots)) >= 64 ? 32 : 16;
+    return kk_max <= 2 && n >= SHRINK_WIDE_ROWS && n / std::max(1u, std::min(n, slots)) >= 64 ? 32 : 16;
 }
 
 template <int XP, int MT>

@@ -30,23 +30,49 @@ int x_planes(int32_t x_type, int32_t y_type) { return x_type == HK_T_F32 && exac
 
 uint32_t max_tiles(uint32_t n, uint32_t groups, uint32_t tile_rows) { return n / tile_rows + std::min(groups, n); }
 
-// Rows a group, on average, up to which a product takes the int8 engine, and
-// the LDS its images may have (two workgroups a CU).
-constexpr uint32_t VEC_ROWS = 4;
+// The shapes' borders, by the rows a group has on average (512 experts of
+// 512 x 2048 and 2048 x 512 Q4, mixed 2048 x 512; both sides in us).
+//
+// The int8 engine streams the weights best but takes each position's image
+// apart anew.  Exact weights (y in f32 or f16): f32 SwiGLU of 4 rows 149, by
+// tiles 212, of 6 rows 203 / 208; mixed product of 4 rows 78 / 92.  Rounded
+// weights (y in bf16): SwiGLU of 2 rows 95 / 101, of 3 rows 124 / 116.
+constexpr uint32_t VEC_ROWS = 4, VEC_ROWS_BF16 = 2;
+// LDS that its images may have: two workgroups a CU.
 constexpr size_t VEC_LDS = 64 * 1024;
+// Its workgroups: few re-read the images less, many fill the CUs evenly (16
+// rows x 10 of 512 experts: 1024 34.2, 2048 32.2, 4096 32.1; mixed product of
+// 64 x 10: 39.4, 37.0, 41.6).
+constexpr uint32_t VEC_GROUPS = 2048;
+// Tiles through LDS read x once for 16 row tiles, but need workgroups enough
+// to hide their latency; the split kernel's time goes with its positions.
+// 16 positions: 6 rows a group, product of 16 / 64 groups (128 / 512
+// workgroups) split 9.0 / 17.9, tiles 11.0 / 15.3; SwiGLU of 512 groups
+// (2048) 170 / 122.  64 positions: 24 rows, 8 / 16 groups (64 / 128) 11.2 /
+// 17.3, tiles 14.0 / 14.6; SwiGLU of 48 rows, 16 / 64 groups (64 / 256) 33 /
+// 96, tiles 41 / 52.  With adapters (4096 x 2048): 128 / 192 rows (32 / 48)
+// 34.9 / 45.7, tiles 37.6 / 39.0; 2048 x 7168: 256 / 512 rows 89 / 147, tiles
+// 100 / 99.
+constexpr uint32_t TILE_GROUPS_16 = 256, TILE_GROUPS_64 = 96, TILE_GROUPS_LORA = 48;
+// Tiles of 128 positions need half the weight decoding of 64 (SwiGLU, 16 rows
+// 145 / 158 of 64-position tiles, 12 rows 151 / 145, 80 rows 260 / 305), and
+// for the short rows of a down projection fewer workgroups to hide the stores
+// (64 rows 180 / 166, 71 rows 184 / 184, 80 rows 191 / 201).
+constexpr uint32_t TILE8_ROWS = 70, TILE8_ROWS_GLU = 15, TILE8_GROUPS = 256;
 
 // The int8 engine wants few rows a group.  (The bound on the source rows makes
 // the workspace of a larger batch enough for every smaller one.)
-bool takes_vec(int kind, int form, uint32_t n, uint32_t groups, uint32_t x_rows, uint32_t cols) {
-    return form != ROWS_LORA && n / std::max(1u, std::min(groups, n)) <= VEC_ROWS && x_rows <= (VEC_ROWS + 1u) * groups &&
+bool takes_vec(int kind, int form, int wp, uint32_t n, uint32_t groups, uint32_t x_rows, uint32_t cols) {
+    return form != ROWS_LORA && n / std::max(1u, std::min(groups, n)) <= (wp == 2 ? VEC_ROWS : VEC_ROWS_BF16) && x_rows <= (VEC_ROWS + 1u) * groups &&
            rows_vec_image_bytes(kind, cols) <= VEC_LDS;
 }
 
-// The launch's shape by the rows a group has on average.
-//  vec    up to 4: the int8 engine, bound by the weight stream
-//  split  up to 16 rows a tile (or too few tiles to fill the device), the
-//         columns over the waves
-//  tile   64 or 128 rows a tile through LDS: bound by the matrix cores
+// The launch's shape:
+//  vec    a few rows a group: the int8 engine, bound by the weight stream
+//  split  16 or 64 positions a workgroup, the columns over its waves: bound by
+//         latency
+//  tile   64 or 128 positions through LDS: bound by the instructions that
+//         decode weights and the matrix cores
 RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t n, uint32_t groups, uint32_t x_rows,
                     uint32_t cols, uint32_t row_tiles) {
     RowsShape sh{};
@@ -54,24 +80,26 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     sh.form = form;
     sh.wp = exact_weights(y_type) ? 2 : 1;
     sh.xp = x_planes(x_type, y_type);
-    if (takes_vec(kind, form, n, groups, x_rows, cols)) {
+    if (takes_vec(kind, form, sh.wp, n, groups, x_rows, cols)) {
         sh.vec = true;
         const size_t img = rows_vec_image_bytes(kind, cols);
         sh.tile_rows = img * 4 <= VEC_LDS ? 4 : img * 2 <= VEC_LDS ? 2 : 1;
-        // a workgroup's row tiles: whole rounds of its waves, and about 2048 workgroups in all
+        // a workgroup's row tiles: whole rounds of its waves, and about VEC_GROUPS workgroups in all
         const uint32_t round = form == ROWS_GLU ? 4 : 8, tiles = std::min(groups, n);
-        const uint32_t most = (uint32_t)(((uint64_t)row_tiles * tiles + 2047u) / 2048u);
+        const uint32_t most = (uint32_t)(((uint64_t)row_tiles * tiles + VEC_GROUPS - 1u) / VEC_GROUPS);
         sh.block_tiles = std::max(1u, (most + round - 1u) / round) * round;
         return sh;
     }
     const uint32_t stages = rows_stages(kind, cols);
     const uint32_t per = n / std::max(1u, std::min(groups, n));
     const bool tile8 = rows_tile8(kind, kind == HK_BIN ? 1 : sh.wp, sh.xp, form);
-    sh.mt = per <= 16 ? 1 : per <= 64 || !tile8 ? 4 : 8;
     const uint32_t blocks = (row_tiles * (form == ROWS_GLU ? 2u : 1u) + 15u) / 16u;
-    const uint32_t tiles = std::max(std::min(groups, n), n / (16u * sh.mt));
-    sh.tile = sh.mt > 1 && (uint64_t)tiles * blocks >= 256;
-    if (!sh.tile && sh.mt > 4) sh.mt = 4;
+    auto groups_of = [&](uint32_t rows) { return (uint64_t)std::max(std::min(groups, n), n / rows) * blocks; };
+    sh.tile = groups_of(64) >= (per <= 16 ? TILE_GROUPS_16 : form == ROWS_LORA ? TILE_GROUPS_LORA : TILE_GROUPS_64);
+    if (sh.tile)
+        sh.mt = tile8 && per > (form == ROWS_GLU ? TILE8_ROWS_GLU : TILE8_ROWS) && groups_of(128) >= TILE8_GROUPS ? 8 : 4;
+    else
+        sh.mt = per <= 16 ? 1 : 4;
     sh.tile_rows = 16u * sh.mt;
     // columns over as many waves as have a superstep each
     const uint32_t supers = (kind == HK_BIN || kind == HK_MIXED) ? stages / 4u : stages;

@@ -106,12 +106,23 @@ def test_ranks(ctx, oracle, max_rank, ranks, x_type, y_type, a_type):
 
 
 @pytest.mark.parametrize("x_type,y_type", TYPES)
+@pytest.mark.parametrize("kind,cols", [("q4", 288), ("q8", 192), ("mixed", 640), ("bin", 512), ("u3", 160)])
+def test_many_rows(ctx, oracle, kind, cols, x_type, y_type):
+    """Rows and outputs enough for the kernel that tiles through LDS."""
+    say("lora many rows of all", kind, x_type, y_type)
+    ranks = [16, 0, 33, 64, 7]
+    ids = _mix(np.random.default_rng(cols), 645, len(ranks))
+    ids[100:400] = 2
+    _run(ctx, oracle, kind, 1100, cols, ids, ranks, 64, x_type, y_type, stride=5)
+
+
+@pytest.mark.parametrize("x_type,y_type", TYPES)
 @pytest.mark.parametrize("ranks,max_rank", [([16, 9], 16), ([64, 33, 5, 0], 64), ([128, 40], 128)])
 def test_many_rows_a_slot(ctx, oracle, ranks, max_rank, x_type, y_type):
-    """Slots of hundreds of rows, and one of a single row among them."""
+    """Slots of hundreds and thousands of rows, and one of a single row among them."""
     say("lora many rows", ranks, x_type, y_type)
     rng = np.random.default_rng(len(ranks))
-    for n in (64 * len(ranks) - 1, 64 * len(ranks), 531):
+    for n in (531, 4200):
         ids = _mix(rng, n, len(ranks))
         ids[ids == len(ranks) - 1] = 0
         ids[n // 2] = len(ranks) - 1

@@ -108,8 +108,7 @@ def _exact_grouped(xe, off, src, ws, x_type, y_type):
 
 
 COUNTS = {
-    # mean rows a group: up to 4 the int8 engine, up to 16 the split kernel, up to 64 the tile kernel with 64 rows, beyond with 128
-    # (64 where two planes are needed); a few tiles alone take the split kernel
+    # mean rows a group: a few the int8 engine, else the split kernel with 16 or 64 positions a workgroup
     "ones": [1, 0, 2, 3, 4, 5, 9, 0, 1, 1],
     "few": [0, 1, 2, 15, 16, 17, 0, 0, 33, 1],
     "mid": [20, 0, 64, 65, 1, 130],
@@ -147,6 +146,86 @@ def test_grouped_product(ctx, oracle, kind, counts, x_type, y_type):
         _check(got[:off[-1]], exact, bound, y_type, (kind, rows, cols, counts))
         assert np.all(got[off[-1]:] == 5.0) and np.all(rest == 5.0)  # rows behind the last group, and what is not a row
         assert ctx.device_status() == 0
+
+
+def _many(rng, mean, groups=130):
+    """Row counts round `mean` with the tiles' edges among them."""
+    cs = rng.poisson(mean, groups)
+    edges = [0, 1, 15, 16, 17, 31, 32, 33, 0, 63, 64, 65, 95, 96, 97, 127, 128, 129, 200, 0]
+    at = rng.permutation(groups)[:len(edges)]
+    cs[at] = edges
+    return [int(c) for c in cs]
+
+
+MANY = {"q4": 416, "q8": 448, "u3": 416, "bin": 640, "mixed": 640}
+
+
+@pytest.mark.parametrize("x_type,y_type", TYPES)
+@pytest.mark.parametrize("mean", [10, 40, 90])
+@pytest.mark.parametrize("kind", sorted(MANY))
+def test_many_groups(ctx, oracle, kind, mean, x_type, y_type):
+    """Workgroups enough for the kernels that tile through LDS (64 positions,
+    and 128 from 70 rows a group on): gathered, strided, with a row that is not
+    finite, indexes outside x and rows behind the last group."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm, RowGroups
+    say("many groups", kind, mean, x_type, y_type)
+    rows, cols = 300, MANY[kind]
+    rng = np.random.default_rng(mean)
+    cs = _many(rng, mean)
+    off = np.concatenate([[0], np.cumsum(cs)]).astype(np.int32)
+    used, n = int(off[-1]), int(off[-1]) + 3
+    made = [R.make_organ(ctx, oracle, kind, rows, cols, 5000 + g) for g in range(3)]
+    pick = [made[g % 3] for g in range(len(cs))]
+    order = rng.permutation(n).astype(np.int32)
+    v = rng.standard_normal((n, cols)).astype(np.float32)
+    bad = rng.permutation(used)[:4]
+    v[order[bad[0]], cols - 1], v[order[bad[1]], 0] = np.nan, np.inf
+    src = order.copy()
+    order[bad[2]], order[bad[3]] = n, -1
+    src[bad[2:]] = 0
+    x, _, xe = R.rows_on(ctx, v, x_type, stride=cols + 8)
+    y, yb, _ = R.rows_on(ctx, np.full((n, rows), 5.0), y_type, stride=rows + 1, lead=1, fill=5.0)
+    plan = RowGroups(ctx, n, len(cs), offsets=ctx.to_device(off), order=ctx.to_device(order))
+    ctx.device_status()
+    GroupedGemm(ctx, OrganSet(ctx, [m[0] for m in pick]), n, x_type, y_type)(x, plan, y, gather=True)
+    assert ctx.device_status() == 3
+    got, rest = R.read_rows(yb, y)
+    assert np.all(got[used:] == 5.0) and np.all(rest == 5.0)
+    assert np.all(np.isnan(got[bad]))
+    ok = np.setdiff1d(np.arange(used), bad)
+    xe = np.where(np.isfinite(xe), xe, 0.0)
+    exact, bound = _exact_grouped(xe, off, src[:used], [m[1] for m in pick], x_type, y_type)
+    _check(got[ok], exact[ok], bound[ok], y_type, (kind, mean))
+
+
+@pytest.mark.parametrize("x_type,y_type", TYPES[:3])
+@pytest.mark.parametrize("mean", [10, 40])
+@pytest.mark.parametrize("kind", sorted(MANY))
+def test_many_groups_swiglu(ctx, oracle, kind, mean, x_type, y_type):
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedSwiGlu, RowGroups
+    say("many groups swiglu", kind, mean, x_type, y_type)
+    rows, cols, per_row = 150, MANY[kind], 3
+    rng = np.random.default_rng(mean + 1)
+    cs = _many(rng, mean)
+    cs += [-sum(cs) % per_row]
+    groups, n = len(cs), sum(cs)
+    ids = rng.permutation(np.repeat(np.arange(groups), cs)).astype(np.int32)
+    gate = [R.make_organ(ctx, oracle, kind, rows, cols, 5100 + g) for g in range(2)]
+    up = [R.make_organ(ctx, oracle, kind, rows, cols, 5200 + g) for g in range(3)]
+    gate, up = [gate[g % 2] for g in range(groups)], [up[g % 3] for g in range(groups)]
+    plan = RowGroups(ctx, n, groups).build(ctx.to_device(ids))
+    off, order, _ = R.group_oracle(ids, groups)
+    x, _, xe = R.rows_on(ctx, rng.standard_normal((n // per_row, cols)) * 2, x_type)
+    y, yb, _ = R.rows_on(ctx, np.full((n, rows), 5.0), y_type)
+    GroupedSwiGlu(ctx, OrganSet(ctx, [m[0] for m in gate]), OrganSet(ctx, [m[0] for m in up]), n // per_row, x_type, y_type)(
+        x, plan, y, gather=True, per_row=per_row)
+    src = order // per_row
+    g, bg = _exact_grouped(xe, off, src, [m[1] for m in gate], x_type, y_type)
+    u, bu = _exact_grouped(xe, off, src, [m[1] for m in up], x_type, y_type)
+    exact = R.silu(g) * u
+    assert np.all(np.abs(R.read_rows(yb, y)[0] - exact) <= R.rounded(R.swiglu_bound(g, bg, u, bu), exact, y_type))
 
 
 @pytest.mark.parametrize("group", [64, 128])
