@@ -1,10 +1,13 @@
 // hk_rows_kernel.h -- the product kernels of hk_rows.h; each kind is
 // instantiated in a translation unit of its own (hk_rows_<kind>.hip).
 //
-// Both kernels multiply a tile of 16 MT positions of one group with row tiles
-// of the group's organ.  The weights are the MFMA's A operand (its 16 rows)
-// and the image the B operand (16 positions), so a lane ends with four
-// consecutive rows of one position.
+// The tile and the split kernel multiply a tile of 16 MT positions of one group
+// with row tiles of the group's organ on the f16 matrix cores.  The weights are
+// the MFMA's A operand (its 16 rows) and the image the B operand (16
+// positions), so a lane ends with four consecutive rows of one position.  The
+// vec kernel takes up to four positions of a group through the int8 GEMV
+// engine.  Which one a call takes, and at what sizes each is faster, is
+// shape_for's (hk_rows_api.cpp).
 #pragma once
 
 #include <type_traits>
@@ -17,7 +20,10 @@ namespace hk {
 // The work item of this workgroup: position tile and row block.  Workgroups
 // go to the 8 XCDs round robin.  With many position tiles an XCD takes every
 // eighth one with all its row blocks in a row, so the blocks that read the
-// same x rows share its L2; with few, the row blocks go round the XCDs.
+// same x rows share its L2 (down projection of 4096 x 10 rows 210 us, adapters
+// over 4096 rows 191, SwiGLU over 32 wide experts 592; with the row blocks
+// round the XCDs 219, 201, 614); with few, the row blocks go round the XCDs, or
+// some would have no work.
 constexpr uint32_t ROWS_XCD_TILES = 32;
 __device__ __forceinline__ void rows_item(const RowsArgs& a, uint32_t* tile, uint32_t* block) {
     if (a.tiles < ROWS_XCD_TILES) {
@@ -133,7 +139,7 @@ __device__ __forceinline__ void rows_each(F&& f) {
     }
 }
 
-// The adapters' part.  Positions with an adapter (those before
+// The adapters' part.  Positions with an adapter (those from offsets[0] to
 // offsets[slots]) are first moved from the units of their x row (2^-exps) to
 // those of their mid row; then B_s mid is added for the slots s with positions
 // in the tile [first, last) -- every kw-th of them where kw waves share the
@@ -229,10 +235,11 @@ __device__ __forceinline__ void rows_lora(const RowsArgs& a, uint32_t first, uin
     const uint32_t m = (uint32_t)lane & 15u, q = (uint32_t)lane >> 4;
     const uint32_t pitch = L.kk_max * 64u * L.planes;
     const uint32_t grouped = __builtin_amdgcn_readfirstlane(h.grouped);
-    if (first >= grouped) return;
+    const uint32_t lowest = __builtin_amdgcn_readfirstlane(h.o0);  // offsets[0]: rows before it have no adapter either
+    if (first >= grouped || last <= lowest) return;
     rows_each<MT>([&](auto mt) {
         const uint32_t p = first + 16u * mt + m;
-        if (p < grouped) {
+        if (p >= lowest && p < grouped) {
             const int32_t g = h.g[mt];
             const bool nan = exps[mt] == ROWS_EXP_BAD || g == ROWS_EXP_BAD;
             const int d = nan ? 0 : g - exps[mt];

@@ -153,6 +153,31 @@ def test_in_order_and_strided(ctx, oracle, n):
     _run(ctx, oracle, "q4", 70, 160, _mix(np.random.default_rng(n), n, 4), [4, 8, 16, 32], 32, "f32", "bf16", stride=3, lead=1)
 
 
+@pytest.mark.parametrize("n", [6, 40, 400])
+def test_rows_before_the_first_slot(ctx, oracle, n):
+    """offsets[0] > 0: the rows before it have no adapter, whatever the workspace holds."""
+    from hawking_amd.rows import LoraBank, LoraGemm, RowGroups
+    say("lora first rows", n)
+    rng = np.random.default_rng(n)
+    rows, cols, k = 48, 128, n // 3
+    w, we = R.make_organ(ctx, oracle, "q4", rows, cols, 8400)
+    bank = LoraBank(ctx, w, 2, 16)
+    a, b, ae, be = _adapter(ctx, rng, 16, rows, cols, "bf16")
+    bank.set(1, 16, a, b)
+    plan = RowGroups(ctx, n, 2, offsets=ctx.to_device(np.array([k, k, n - 1], np.int32)))
+    x, _, xe = R.rows_on(ctx, rng.standard_normal((n, cols)), "f32")
+    y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+    gemm = LoraGemm(ctx, w, bank, n)
+    ctx.device_status()
+    for _ in range(2):
+        gemm.ws.upload(np.full(gemm.ws.shape, 0x7F, np.uint8))
+        gemm(x, plan, y, in_order=True)
+        want = xe @ we.T
+        want[k:n - 1] += xe[k:n - 1] @ ae.T @ be.T
+        got = R.read_rows(yb, y)[0]
+        assert ctx.device_status() == 0 and np.linalg.norm(got - want) <= 2e-5 * np.linalg.norm(want)
+
+
 def test_slots_are_replaced_and_emptied(ctx, oracle):
     from hawking_amd.rows import LoraBank, LoraGemm, RowGroups
     rng = np.random.default_rng(9)
