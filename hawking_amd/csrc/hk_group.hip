@@ -93,7 +93,9 @@ __global__ void __launch_bounds__(64 * NW) group_count_kernel(const int32_t* __r
 // their own ids in LDS (16-bit counters, two a word), the counts of the
 // waves before give each wave its first place of a key, and the wave then
 // walks its ids 64 at a time: equal lanes find each other by one ballot a bit
-// of the key, and the lowest of them advances the counter.
+// of the key, and the lowest of them advances the counter.  327,680 ids of 512
+// groups: counts 2.6 us, places 10.6, of which 2.7 are the parts' counts and 1
+// the ballots and the scattered stores; the rest is latency between barriers.
 template <int NW>
 __global__ void __launch_bounds__(64 * NW) group_place_kernel(const int32_t* __restrict__ ids, uint32_t n, uint32_t G,
                                                               uint32_t bits, const uint32_t* __restrict__ part,
@@ -282,7 +284,9 @@ __device__ __forceinline__ void put_elem(void* y, int type, size_t at, float v) 
 
 // y_t = base_t + sum over r ascending of w[t, r] x[pos[t, r]] in f32, one
 // rounding: V columns a thread, the x rows of CHUNK routes in flight at once.
-// A position outside [0, n) adds nothing.  Bound by reading x once.
+// A position outside [0, n) adds nothing.  Bound by reading x once: 8192 x 10
+// bf16 rows of 2048 88 us, 4.5 TB/s of the 4.9 that a copy reaches; 32 x 8 f32
+// rows of 7168 3.8 us.
 template <int TYPE, int V>
 __global__ void __launch_bounds__(256) combine_kernel(const void* x, size_t xs, uint32_t n, const int32_t* __restrict__ pos,
                                                       const float* __restrict__ w, uint32_t K, uint32_t cols,

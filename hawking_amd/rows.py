@@ -41,6 +41,13 @@ def _dp(a):
     return getattr(a, "ptr", a)
 
 
+def _holds(a, elements: int, itemsize: int, what: str) -> None:
+    """Refuses a buffer whose size is known and too small."""
+    size = getattr(a, "nbytes", None)
+    if size is not None and size < elements * itemsize:
+        raise ValueError(f"{what} has {size} bytes, the call needs {elements * itemsize}")
+
+
 class Rows:
     """n rows of `cols` elements of a device buffer (a DeviceArray, an object
     with a .ptr, or a c_void_p), `stride` elements apart."""
@@ -48,6 +55,8 @@ class Rows:
     def __init__(self, buf, n: int, cols: int, dtype: str = "f32", stride: int | None = None):
         self.buf, self.n, self.cols, self.dtype = buf, int(n), int(cols), dtype
         self.stride = self.cols if stride is None else int(stride)
+        if self.n:
+            _holds(buf, (self.n - 1) * self.stride + self.cols, 4 if dtype == "f32" else 2, "the rows' buffer")
         self.src = RowsSrc(_dp(buf), _row_type(dtype), self.n, self.stride)
         self.ref = C.byref(self.src)
 
@@ -70,10 +79,13 @@ class RowGroups:
         self.offsets = ctx.empty(self.n_groups + 1, np.int32) if offsets is None else offsets
         self.order = ctx.empty(self.n, np.int32) if order is None else order
         self.pos = ctx.empty(self.n, np.int32) if pos is None else pos
+        for a, k, what in ((self.offsets, self.n_groups + 1, "offsets"), (self.order, self.n, "order"), (self.pos, self.n, "pos")):
+            _holds(a, k, 4, what)
         self.ws_bytes = int(ctx.L.hk_group_rows_workspace(self.n, self.n_groups))
         self.ws = ctx.empty(self.ws_bytes, np.uint8) if self.ws_bytes else None
 
     def build(self, ids, stream=None) -> "RowGroups":
+        _holds(ids, self.n, 4, "ids")
         self.ctx.call("hk_group_rows", _dp(ids), self.n, self.n_groups, _dp(self.offsets), _dp(self.order), _dp(self.pos),
                       _dp(self.ws), self.ws_bytes, stream if stream is not None else self.ctx.stream)
         return self
@@ -86,9 +98,11 @@ class _Product:
         self.ctx, self.rows, self.cols = ctx, rows, cols
         self.x_type, self.y_type = x_type, y_type
         _row_type(x_type), _row_type(y_type)
-        self.ws, self.ws_bytes, self._fits = None, 0, None
+        self.ws, self.ws_bytes, self._fits, self._kept = None, 0, None, []
 
-    def _check(self, x: Rows, y: Rows, size) -> None:
+    def _check(self, x: Rows, groups: RowGroups, n_groups: int, y: Rows, size) -> None:
+        if groups.n != y.n or groups.n_groups != n_groups:
+            raise ValueError(f"{groups.n} positions of {groups.n_groups} groups given for {y.n} rows of {n_groups}")
         if x.dtype != self.x_type or y.dtype != self.y_type:
             raise ValueError(f"rows of {x.dtype} -> {y.dtype} given to a product of {self.x_type} -> {self.y_type}")
         if x.cols != self.cols or y.cols != self.rows:
@@ -96,8 +110,8 @@ class _Product:
         if self._fits != (x.n, y.n):
             need = int(size(x.n, y.n))
             if need > self.ws_bytes:
-                # calls of the old workspace may be in flight
-                self.ctx.device_synchronize()
+                # calls of the old workspace may be in flight, or captured in a graph
+                self._kept.append(self.ws)
                 self.ws = self.ctx.empty(need, np.uint8)
                 self.ws_bytes = need
             self._fits = (x.n, y.n)
@@ -106,7 +120,8 @@ class _Product:
 class GroupedGemm(_Product):
     """y_p = W_g x_p over the organs of a set (hk_gemm_grouped), for rows of
     x_type -> y_type; the workspace is made for max_rows rows of x, gathered
-    or in grouped order, and grows (synchronising) where a call needs more."""
+    or in grouped order, and another is made where a call needs more (the old
+    one is kept: a captured graph may hold it)."""
 
     def __init__(self, ctx: Context, organs: OrganSet, max_rows: int, x_type: str = "f32", y_type: str = "f32"):
         self.organs = organs
@@ -122,7 +137,7 @@ class GroupedGemm(_Product):
 
     def __call__(self, x: Rows, groups: RowGroups, y: Rows, gather: bool = False, per_row: int = 1, stream=None) -> None:
         """gather: position p reads x row order[p] / per_row, else row p."""
-        self._check(x, y, self._size)
+        self._check(x, groups, len(self.organs.organs), y, self._size)
         self.ctx.call("hk_gemm_grouped", self.organs.h, x.ref, _dp(groups.order) if gather else None, per_row,
                       _dp(groups.offsets), y.ref, self.ws.ptr, self.ws_bytes,
                       stream if stream is not None else self.ctx.stream)
@@ -138,7 +153,7 @@ class GroupedSwiGlu(GroupedGemm):
         super().__init__(ctx, gate, max_rows, x_type, y_type)
 
     def __call__(self, x: Rows, groups: RowGroups, y: Rows, gather: bool = False, per_row: int = 1, stream=None) -> None:
-        self._check(x, y, self._size)
+        self._check(x, groups, len(self.organs.organs), y, self._size)
         self.ctx.call("hk_gemm_grouped_swiglu", self.organs.h, self.up.h, x.ref, _dp(groups.order) if gather else None,
                       per_row, _dp(groups.offsets), y.ref, self.ws.ptr, self.ws_bytes,
                       stream if stream is not None else self.ctx.stream)
@@ -148,6 +163,10 @@ def combine_rows(ctx: Context, x: Rows, pos, weights, per_row: int, y: Rows, bas
     """y_t = base_t + sum_r weights[t, r] x[pos[t, r]] (hk_combine_rows); base may be y."""
     if x.cols != y.cols or (base is not None and base.cols != y.cols):
         raise ValueError("x, base and y must have rows of one length")
+    if base is not None and base.n < y.n:
+        raise ValueError("base must have the rows of y")
+    _holds(pos, y.n * per_row, 4, "pos")
+    _holds(weights, y.n * per_row, 4, "weights")
     ctx.call("hk_combine_rows", x.ref, _dp(pos), _dp(weights), per_row, y.cols, base.ref if base is not None else None,
              y.ref, stream if stream is not None else ctx.stream)
 
@@ -165,6 +184,9 @@ class LoraBank:
 
     def set(self, slot: int, rank: int, a, b, dtype: str = "bf16", scale: float = 1.0, stream=None) -> None:
         """Adapter scale * B A from device arrays a [rank, cols] and b [rows, rank]; rank 0 empties the slot."""
+        if rank:
+            _holds(a, rank * self.cols, 4 if dtype == "f32" else 2, "a")
+            _holds(b, self.rows * rank, 4 if dtype == "f32" else 2, "b")
         self.ctx.call("hk_lora_bank_set", self.h, slot, rank, _dp(a), _dp(b), _row_type(dtype), scale,
                       stream if stream is not None else self.ctx.stream)
 
@@ -197,7 +219,7 @@ class LoraGemm(_Product):
 
     def __call__(self, x: Rows, groups: RowGroups, y: Rows, in_order: bool = False, stream=None) -> None:
         """in_order: the rows are in grouped order already."""
-        self._check(x, y, self._size)
+        self._check(x, groups, self.bank.n_slots, y, self._size)
         self.ctx.call("hk_gemm_lora", self.organ.h, self.bank.h, x.ref, None if in_order else _dp(groups.order),
                       _dp(groups.offsets), y.ref, self.ws.ptr, self.ws_bytes,
                       stream if stream is not None else self.ctx.stream)

@@ -673,7 +673,7 @@ typedef struct hk_rows {
  *                          offsets[n_groups] on
  *   pos[n]                 the position of index i, -1 for an id outside
  * All device int32; ids must not overlap the outputs.  ws: device memory of
- * hk_group_rows_workspace(n, n_groups) bytes (0 for few ids: ws may be NULL),
+ * hk_group_rows_workspace(n, n_groups) bytes (0 up to 8192 ids: ws may be NULL),
  * written by the call.  n may be 0 (offsets are written).  Limits
  * (HK_E_UNSUPPORTED beyond): n < 2^31, 1 <= n_groups <= 8192. */
 size_t hk_group_rows_workspace(uint32_t n, uint32_t n_groups);
@@ -690,10 +690,11 @@ int hk_group_rows(hk_ctx* ctx, const int32_t* ids, uint32_t n, uint32_t n_groups
  * are not written.  A position whose r is not below x->n gives NaN and latches
  * HK_E_ROUTE's device bit; offsets outside [0, n] are clamped.  x and y must
  * not overlap.  Every kind but HK_F32 and HGRAVR02 (HK_E_UNSUPPORTED).  The
- * weights of a group are read once for every 128 of its rows (64 or 16 where
- * groups are small).  ws: 256-byte aligned device memory of
- * hk_gemm_grouped_workspace bytes that no other call uses meanwhile (calls on
- * two streams, or two captured graphs that may run at once, need one each). */
+ * weights of a group are read once for every 128 of its rows (64, 16 or 4 where
+ * groups have few).  ws: 256-byte aligned device memory of
+ * hk_gemm_grouped_workspace bytes, which is enough for every call of as many
+ * rows or fewer, that no other call uses meanwhile (calls on two streams, or
+ * two captured graphs that may run at once, need one each). */
 size_t hk_gemm_grouped_workspace(const hk_organ_set* set, uint32_t x_rows, int32_t x_type, uint32_t n, int32_t y_type);
 int hk_gemm_grouped(hk_ctx* ctx, const hk_organ_set* set, const hk_rows* x, const int32_t* order, uint32_t per_row,
                     const int32_t* offsets, const hk_rows* y, void* ws, size_t ws_bytes, hk_stream stream);
@@ -730,7 +731,8 @@ int hk_lora_bank_set(hk_ctx* ctx, hk_lora_bank* bank, uint32_t slot, uint32_t ra
 /* y_i = W x_i + scale_s B_s (A_s x_i), s the adapter of row i: hk_group_rows
  * over the rows' adapter ids with n_groups = the bank's n_slots gives offsets
  * and order (rows with an id outside, say -1, have no adapter: y_i = W x_i);
- * order NULL: the rows are in grouped order already.  x->n = y->n rows; x and
+ * order NULL: the rows are in grouped order already (those before offsets[0]
+ * and from offsets[n_slots] on have no adapter).  x->n = y->n rows; x and
  * y in the batch's own order, not overlapping.  order must be a permutation
  * (an index outside the rows is dropped and latches HK_E_ROUTE's device bit).
  * ws as in hk_gemm_grouped, hk_gemm_lora_workspace bytes. */

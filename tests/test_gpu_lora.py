@@ -259,7 +259,13 @@ def test_lora_refusals(ctx, oracle):
     y, _, _ = R.rows_on(ctx, np.zeros((4, 32)), "f32")
     y3, _, _ = R.rows_on(ctx, np.zeros((3, 32)), "f32")
     gemm = LoraGemm(ctx, w, bank, 4)
-    assert code(lambda: gemm(x, plan, y3)) == HK_E_GEOMETRY
+    assert code(lambda: gemm(x, RowGroups(ctx, 3, 2).build(ctx.to_device(np.zeros(3, np.int32))), y3)) == HK_E_GEOMETRY
+    with pytest.raises(ValueError):
+        gemm(x, plan, y3)
+    with pytest.raises(ValueError):
+        gemm(x, RowGroups(ctx, 4, 1).build(ctx.to_device(np.zeros(4, np.int32))), y)  # a bank of two slots
+    with pytest.raises(ValueError):
+        bank.set(0, 16, ctx.empty(16 * 128 - 1, np.uint16), d)
     other = R.make_organ(ctx, oracle, "q4", 32, 160, 8301)[0]
     assert code(lambda: ctx.call("hk_gemm_lora", other.h, bank.h, x.ref, None, plan.offsets.ptr, y.ref, gemm.ws.ptr,
                                  gemm.ws_bytes, None)) == HK_E_GEOMETRY

@@ -407,7 +407,7 @@ def test_wild_indexes_stay_inside(ctx, oracle, n):
 def test_product_refusals(ctx, oracle):
     from hawking_amd._lib import HK_E_GEOMETRY, HK_E_INVALID_ARG, HK_E_UNSUPPORTED, HawkingError
     from hawking_amd.organs import DenseF32Organ, OrganSet, SyntheticOrgan
-    from hawking_amd.rows import GroupedGemm, GroupedSwiGlu, Rows
+    from hawking_amd.rows import GroupedGemm, GroupedSwiGlu, Rows, combine_rows
     w = R.make_organ(ctx, oracle, "q4", 32, 128, 3400)[0]
     s = OrganSet(ctx, [w])
     plan, _, _ = _plan(ctx, [4])
@@ -437,6 +437,17 @@ def test_product_refusals(ctx, oracle):
         gemm(Rows(x.buf, 4, 128, "bf16"), plan, y)
     with pytest.raises(ValueError):
         gemm(Rows(x.buf, 4, 64, "f32"), plan, y)
+    # a plan of other groups or rows: its offsets would be read past their end
+    with pytest.raises(ValueError):
+        gemm(x, _plan(ctx, [2, 2])[0], y)
+    with pytest.raises(ValueError):
+        gemm(x, _plan(ctx, [3])[0], y)
+    with pytest.raises(ValueError):
+        Rows(ctx.empty((4, 128)), 5, 128)
+    with pytest.raises(ValueError):
+        plan.build(ctx.to_device(np.zeros(3, np.int32)))
+    with pytest.raises(ValueError):
+        combine_rows(ctx, x, plan.pos, ctx.empty(7), 2, x)
     with pytest.raises(ValueError):
         GroupedSwiGlu(ctx, s, OrganSet(ctx, [R.make_organ(ctx, oracle, "q4", 16, 128, 3402)[0]]), 4)
 
@@ -600,6 +611,39 @@ def test_captured_block(ctx, oracle, tokens):
         calls(eager)
         ctx.synchronize(stream)
         assert np.array_equal(cap["out"].download(stream), eager["out"].download(stream)), k
+    g.free()
+
+
+def test_captured_product_keeps_its_workspace(ctx, oracle):
+    """A larger eager call of the same object between a graph's replays."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    say("captured product, larger call")
+    rows, cols = 48, 256
+    s = OrganSet(ctx, [R.make_organ(ctx, oracle, "q4", rows, cols, 7100 + g)[0] for g in range(2)])
+    stream = ctx.new_stream()
+    gemm = GroupedGemm(ctx, s, 20, "bf16", "f32")
+    made = []
+    for counts in ([12, 8], [700, 900]):
+        plan, _, n = _plan(ctx, counts)
+        x, xb, _ = R.rows_on(ctx, np.random.default_rng(n).standard_normal((n, cols)), "bf16")
+        y, yb, _ = R.rows_on(ctx, np.zeros((n, rows)), "f32")
+        made.append((plan, x, y, yb))
+    (plan, x, y, yb), (plan2, x2, y2, _) = made
+    gemm(x, plan, y, stream=stream)
+    ctx.synchronize(stream)
+    want = yb.download(stream)
+    g = _Graph(ctx, stream)
+    with g:
+        gemm(x, plan, y, stream=stream)
+    for k in range(3):
+        gemm(x2, plan2, y2, stream=stream)
+        other = ctx.to_device(np.full(1 << 20, 0x55, np.uint8))  # where a freed workspace would be
+        yb.upload(np.zeros_like(want), stream)
+        g.replay()
+        ctx.synchronize(stream)
+        assert np.array_equal(yb.download(stream), want), k
+        assert np.all(other.download() == 0x55)
     g.free()
 
 
