@@ -264,6 +264,7 @@ struct RowsShape {
     int form;         // ROWS_PLAIN, ROWS_GLU, ROWS_LORA
     int mt;           // 16-row tiles of positions
     bool tile;        // the tile kernel (x in LDS), else the split kernel
+    int rt;           // tile kernel: row tiles of a wave
     uint32_t kw;      // split kernel: waves that share a row tile's columns
     bool vec;         // the int8 engine: tile_rows positions a tile, block_tiles row tiles a workgroup
     uint32_t tile_rows, block_tiles;

@@ -44,21 +44,30 @@ constexpr size_t VEC_LDS = 64 * 1024;
 // rows x 10 of 512 experts: 1024 34.2, 2048 32.2, 4096 32.1; mixed product of
 // 64 x 10: 39.4, 37.0, 41.6).
 constexpr uint32_t VEC_GROUPS = 2048;
-// Tiles through LDS read x once for 16 row tiles, but need workgroups enough
+// Tiles through LDS read x once for many row tiles, but need workgroups enough
 // to hide their latency; the split kernel's time goes with its positions.
-// 16 positions: 6 rows a group, product of 16 / 64 groups (128 / 512
-// workgroups) split 9.0 / 17.9, tiles 11.0 / 15.3; SwiGLU of 512 groups
-// (2048) 170 / 122.  64 positions: 24 rows, 8 / 16 groups (64 / 128) 11.2 /
-// 17.3, tiles 14.0 / 14.6; SwiGLU of 48 rows, 16 / 64 groups (64 / 256) 33 /
-// 96, tiles 41 / 52.  With adapters (4096 x 2048): 128 / 192 rows (32 / 48)
-// 34.9 / 45.7, tiles 37.6 / 39.0; 2048 x 7168: 256 / 512 rows 89 / 147, tiles
-// 100 / 99.
-constexpr uint32_t TILE_GROUPS_16 = 256, TILE_GROUPS_64 = 96, TILE_GROUPS_LORA = 48;
-// Tiles of 128 positions need half the weight decoding of 64 (SwiGLU, 16 rows
-// 145 / 158 of 64-position tiles, 12 rows 151 / 145, 80 rows 260 / 305), and
-// for the short rows of a down projection fewer workgroups to hide the stores
-// (64 rows 180 / 166, 71 rows 184 / 184, 80 rows 191 / 201).
-constexpr uint32_t TILE8_ROWS = 70, TILE8_ROWS_GLU = 15, TILE8_GROUPS = 256;
+// (Workgroups counted as 64 positions x 16 row tiles.)  16 positions: 10 rows a
+// group, product of 8 / 32 groups (64 / 256 workgroups) split 8.8 / 12.9, tiles
+// 9.2 / 10.9; SwiGLU of 8 / 32 (32 / 128) 11.7 / 18.3, tiles 15.5 / 17.3.  64
+// positions: 24 rows, product of 8 groups (64) 11.3 / 11.2, SwiGLU of 8 / 32 (32
+// / 128) 15.4 / 39.7, tiles 20.6 / 23.1.  With adapters, 4096 x 2048 Q4: 64 / 128
+// rows (16 / 32) 23.7 / 34.9, tiles 28.1 / 28.8; 2048 x 7168: 128 / 256 rows (16
+// / 32) 57 / 87, tiles 71 / 73.
+constexpr uint32_t TILE_GROUPS_16 = 128, TILE_GROUPS_64 = 48, TILE_GROUPS_LORA = 24;
+// Up to two workgroups a CU, twice as many with half the row tiles overlap each
+// other's latency: adapters 4096 x 2048 of 256 / 1024 rows (64 / 256) 29.4 /
+// 42.3 for 38.0 / 43.8, of 4096 rows x 2048 x 7168 (512) 183 for 179; product of
+// 60 rows of 32 / 128 / 512 groups (256 / 1024 / 4096) 19.2 / 42.9 / 176 for
+// 22.0 / 42.9 / 156.  Mixed organs' four row tiles do not fit the registers
+// (512 groups of 60 rows 210 for 241).
+constexpr uint32_t TILE_RT4_GROUPS = 512;
+// Tiles of 128 positions need half the weight decoding of 64: SwiGLU of 16 rows
+// of 512 groups 145 for 158 (12 rows 151 for 145), 80 rows 260 for 305, of 60
+// rows of 64 / 128 groups (256 / 512 workgroups of 128) 51.5 / 77.3 for 42.1 /
+// 78.7, of 200 rows of 32 / 64 (200 / 400) 70 / 97 for 54 / 114.  The short rows
+// of a down projection gain less: 64 rows of 512 groups 180 for 166, 80 rows 191
+// for 201; 80 rows of 128 / 256 groups (1024 / 2048) 58.6 / 97.9 for 52.0 / 98.0.
+constexpr uint32_t TILE8_ROWS = 70, TILE8_ROWS_GLU = 15, TILE8_GROUPS = 2048, TILE8_GROUPS_GLU = 384;
 
 // The int8 engine wants few rows a group.  (The bound on the source rows makes
 // the workspace of a larger batch enough for every smaller one.)
@@ -97,9 +106,10 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     auto groups_of = [&](uint32_t rows) { return (uint64_t)std::max(std::min(groups, n), n / rows) * blocks; };
     sh.tile = groups_of(64) >= (per <= 16 ? TILE_GROUPS_16 : form == ROWS_LORA ? TILE_GROUPS_LORA : TILE_GROUPS_64);
     if (sh.tile)
-        sh.mt = tile8 && per > (form == ROWS_GLU ? TILE8_ROWS_GLU : TILE8_ROWS) && groups_of(128) >= TILE8_GROUPS ? 8 : 4;
+        sh.mt = tile8 && per > (form == ROWS_GLU ? TILE8_ROWS_GLU : TILE8_ROWS) && groups_of(128) >= (form == ROWS_GLU ? TILE8_GROUPS_GLU : TILE8_GROUPS) ? 8 : 4;
     else
         sh.mt = per <= 16 ? 1 : 4;
+    sh.rt = sh.mt == 4 && (kind == HK_MIXED || groups_of(64) < TILE_RT4_GROUPS) ? 2 : 4;
     sh.tile_rows = 16u * sh.mt;
     // columns over as many waves as have a superstep each
     const uint32_t supers = (kind == HK_BIN || kind == HK_MIXED) ? stages / 4u : stages;

@@ -373,9 +373,9 @@ __device__ __forceinline__ void rows_store_tile(const RowsArgs& a, uint32_t firs
     if (__ballot(fin != fin) && lane == 0) atomicOr(a.status, ROWS_ERR_NONFINITE);
 }
 
-// A tile of 16 MT positions x this workgroup's 16 row tiles.
+// A tile of 16 MT positions x this workgroup's 4 RT row tiles.
 //
-// Four waves, four row tiles each (SwiGLU: two gate and two up).  Per stage
+// Four waves, RT row tiles each (SwiGLU: half of them gate, half up).  Per stage
 // (128 columns) the positions' image is copied straight into one of two LDS
 // buffers while the other is multiplied, with one barrier a stage; each wave
 // decodes its own weights in registers, fetched a superstep ahead, so a
@@ -388,10 +388,10 @@ __device__ __forceinline__ void rows_store_tile(const RowsArgs& a, uint32_t firs
 // 491, where storing y in bf16 alone is 34.  The 16-byte chunks of
 // a row are stored at chunk ^ (row % 16), so the 16 rows that a fragment read
 // touches lie in 16 different bank groups.
-template <int KIND, int WP, int XP, int MT, int FORM>
+template <int KIND, int WP, int XP, int MT, int FORM, int RT>
 __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uint32_t first, uint32_t last, uint32_t block,
                                           uint8_t* lds, RowsMap* map) {
-    constexpr int RT = 4, BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
+    constexpr int BM = 16 * MT, STG = RowsCfg<KIND>::STAGES;
     constexpr bool GLU = FORM == ROWS_GLU;
     constexpr uint32_t BUF = BM * 256u * XP;
     const int lane = threadIdx.x & 63;
@@ -499,14 +499,6 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
                 }
 #pragma unroll
                 for (int r = 0; r < RT; ++r) acc[mt][r] = rows_mfma<WP, XP>(wh[u & 1][r], wl[u & 1][r], x[i % (AHEAD + 1)], acc[mt][r]);
-#ifdef ROWS_SCHED
-                __builtin_amdgcn_sched_group_barrier(0x100, XP, 0);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, ROWS_SCHED, 0);
-                }
-#endif
             });
             rows_copied();
             __syncthreads();
@@ -531,8 +523,14 @@ __device__ __forceinline__ void rows_tile(const RowsArgs& a, uint32_t group, uin
     rows_store_tile<MT, RT, GLU>(a, first, last, T0, lane, map, lds + wave * ROWS_OUT_BYTES, exps, acc);
 }
 
-template <int KIND, int WP, int XP, int MT, int FORM>
-__global__ void __launch_bounds__(256, MT == 4 && WP == 1 && XP == 1 && KIND != HK_MIXED && KIND != HK_Q8 ? 3 : 2) rows_tile_kernel(RowsArgs a) {
+// Workgroups a CU by registers: what is resident hides the stages' latency.
+constexpr int rows_tile_resident(int kind, int wp, int xp, int mt, int rt) {
+    if (rt == 2) return xp == 2 ? 2 : kind == HK_MIXED || kind == HK_Q8 ? 3 : 4;
+    if (kind == HK_Q8 || mt == 8) return 2;
+    return wp == 1 && xp == 1 ? 3 : 2;
+}
+template <int KIND, int WP, int XP, int MT, int FORM, int RT>
+__global__ void __launch_bounds__(256, rows_tile_resident(KIND, WP, XP, MT, RT)) rows_tile_kernel(RowsArgs a) {
     constexpr int BM = 16 * MT;
     extern __shared__ __align__(16) uint8_t lds[];  // two buffers of BM x 256 XP bytes
     __shared__ RowsMap map[BM];
@@ -542,13 +540,13 @@ __global__ void __launch_bounds__(256, MT == 4 && WP == 1 && XP == 1 && KIND != 
     // a tile that is not full costs its 32s of positions
     const uint32_t mts = (last - first + 15u) / 16u;
     if constexpr (MT == 8) {
-        if (mts > 6u) rows_tile<KIND, WP, XP, 8, FORM>(a, group, first, last, block, lds, map);
-        else if (mts > 4u) rows_tile<KIND, WP, XP, 6, FORM>(a, group, first, last, block, lds, map);
-        else if (mts > 2u) rows_tile<KIND, WP, XP, 4, FORM>(a, group, first, last, block, lds, map);
-        else rows_tile<KIND, WP, XP, 2, FORM>(a, group, first, last, block, lds, map);
+        if (mts > 6u) rows_tile<KIND, WP, XP, 8, FORM, RT>(a, group, first, last, block, lds, map);
+        else if (mts > 4u) rows_tile<KIND, WP, XP, 6, FORM, RT>(a, group, first, last, block, lds, map);
+        else if (mts > 2u) rows_tile<KIND, WP, XP, 4, FORM, RT>(a, group, first, last, block, lds, map);
+        else rows_tile<KIND, WP, XP, 2, FORM, RT>(a, group, first, last, block, lds, map);
     } else {
-        if (mts > 2u) rows_tile<KIND, WP, XP, 4, FORM>(a, group, first, last, block, lds, map);
-        else rows_tile<KIND, WP, XP, 2, FORM>(a, group, first, last, block, lds, map);
+        if (mts > 2u) rows_tile<KIND, WP, XP, 4, FORM, RT>(a, group, first, last, block, lds, map);
+        else rows_tile<KIND, WP, XP, 2, FORM, RT>(a, group, first, last, block, lds, map);
     }
 }
 
@@ -927,10 +925,10 @@ hipError_t launch_rows_vec_image_kind(const void* x, int type, size_t stride, ui
 
 // ------------------------------------------------------------------ launch
 
-template <int KIND, int WP, int XP, int MT, int FORM>
+template <int KIND, int WP, int XP, int MT, int FORM, int RT>
 hipError_t rows_go_tile(RowsArgs a, hipStream_t s) {
     const uint32_t tiles = FORM == ROWS_LORA ? (a.n + 16u * MT - 1u) / (16u * MT) : a.ws.max_tiles;
-    return rows_launch(rows_tile_kernel<KIND, WP, XP, MT, FORM>, tiles, FORM == ROWS_GLU ? 8u : 16u, 256u, 2u * 16u * MT * 256u * XP, a, s);
+    return rows_launch(rows_tile_kernel<KIND, WP, XP, MT, FORM, RT>, tiles, (FORM == ROWS_GLU ? 2u : 4u) * RT, 256u, 2u * 16u * MT * 256u * XP, a, s);
 }
 
 template <int KIND, int WP, int XP, int MT, int FORM, int RT>
@@ -944,9 +942,11 @@ template <int KIND, int WP, int XP, int FORM>
 hipError_t rows_mt(const RowsShape& sh, const RowsArgs& a, hipStream_t s) {
     constexpr int RT = FORM == ROWS_LORA ? 1 : 2;
     if (sh.tile) {
-        if (sh.mt == 4) return rows_go_tile<KIND, WP, XP, 4, FORM>(a, s);
+        if (sh.mt == 4 && sh.rt == 2) return rows_go_tile<KIND, WP, XP, 4, FORM, 2>(a, s);
+        if constexpr (KIND != HK_MIXED)
+            if (sh.mt == 4) return rows_go_tile<KIND, WP, XP, 4, FORM, 4>(a, s);
         if constexpr (rows_tile8(KIND, WP, XP, FORM))
-            if (sh.mt == 8) return rows_go_tile<KIND, WP, XP, 8, FORM>(a, s);
+            if (sh.mt == 8) return rows_go_tile<KIND, WP, XP, 8, FORM, 4>(a, s);
     } else {
         if (sh.mt == 1) return rows_go_split<KIND, WP, XP, 1, FORM, RT>(sh, a, s);
         if (sh.mt == 4) return rows_go_split<KIND, WP, XP, 4, FORM, RT>(sh, a, s);

@@ -106,12 +106,13 @@ def test_ranks(ctx, oracle, max_rank, ranks, x_type, y_type, a_type):
 
 
 @pytest.mark.parametrize("x_type,y_type", TYPES)
+@pytest.mark.parametrize("n", [645, 6605])
 @pytest.mark.parametrize("kind,cols", [("q4", 288), ("q8", 192), ("mixed", 640), ("bin", 512), ("u3", 160)])
-def test_many_rows(ctx, oracle, kind, cols, x_type, y_type):
-    """Rows and outputs enough for the kernel that tiles through LDS."""
-    say("lora many rows of all", kind, x_type, y_type)
+def test_many_rows(ctx, oracle, kind, cols, n, x_type, y_type):
+    """Rows and outputs enough for the kernel that tiles through LDS, with two and with four row tiles a wave."""
+    say("lora many rows of all", kind, n, x_type, y_type)
     ranks = [16, 0, 33, 64, 7]
-    ids = _mix(np.random.default_rng(cols), 645, len(ranks))
+    ids = _mix(np.random.default_rng(cols), n, len(ranks))
     ids[100:400] = 2
     _run(ctx, oracle, kind, 1100, cols, ids, ranks, 64, x_type, y_type, stride=5)
 

@@ -161,18 +161,18 @@ MANY = {"q4": 416, "q8": 448, "u3": 416, "bin": 640, "mixed": 640}
 
 
 @pytest.mark.parametrize("x_type,y_type", TYPES)
-@pytest.mark.parametrize("mean", [10, 40, 90])
+@pytest.mark.parametrize("mean,groups", [(10, 130), (40, 130), (40, 260), (90, 130)])
 @pytest.mark.parametrize("kind", sorted(MANY))
-def test_many_groups(ctx, oracle, kind, mean, x_type, y_type):
-    """Workgroups enough for the kernels that tile through LDS (64 positions,
-    and 128 from 70 rows a group on): gathered, strided, with a row that is not
+def test_many_groups(ctx, oracle, kind, mean, groups, x_type, y_type):
+    """Workgroups enough for the kernels that tile through LDS, with two and
+    with four row tiles a wave: gathered, strided, with a row that is not
     finite, indexes outside x and rows behind the last group."""
     from hawking_amd.organs import OrganSet
     from hawking_amd.rows import GroupedGemm, RowGroups
-    say("many groups", kind, mean, x_type, y_type)
+    say("many groups", kind, mean, groups, x_type, y_type)
     rows, cols = 300, MANY[kind]
     rng = np.random.default_rng(mean)
-    cs = _many(rng, mean)
+    cs = _many(rng, mean, groups)
     off = np.concatenate([[0], np.cumsum(cs)]).astype(np.int32)
     used, n = int(off[-1]), int(off[-1]) + 3
     made = [R.make_organ(ctx, oracle, kind, rows, cols, 5000 + g) for g in range(3)]
@@ -199,16 +199,40 @@ def test_many_groups(ctx, oracle, kind, mean, x_type, y_type):
     _check(got[ok], exact[ok], bound[ok], y_type, (kind, mean))
 
 
+@pytest.mark.parametrize("x_type", ["bf16", "f32"])
+@pytest.mark.parametrize("kind,cols", [("q4", 160), ("u3", 96), ("bin", 128)])
+def test_wide_product(ctx, oracle, kind, cols, x_type):
+    """Rows and outputs enough for tiles of 128 positions without a gate."""
+    from hawking_amd.organs import OrganSet
+    from hawking_amd.rows import GroupedGemm
+    say("wide product", kind, x_type)
+    rows, groups = 4100, 122
+    rng = np.random.default_rng(cols)
+    cs = _many(rng, 75, groups)
+    made = [R.make_organ(ctx, oracle, kind, rows, cols, 5300 + g) for g in range(2)]
+    pick = [made[g % 2] for g in range(groups)]
+    plan, off, n = _plan(ctx, cs, extra=2)
+    assert n // groups > 70
+    x, _, xe = R.rows_on(ctx, rng.standard_normal((n, cols)), x_type)
+    y, yb, _ = R.rows_on(ctx, np.full((n, rows), 5.0), "bf16")
+    GroupedGemm(ctx, OrganSet(ctx, [m[0] for m in pick]), n, x_type, "bf16")(x, plan, y)
+    got = R.read_rows(yb, y)[0]
+    exact, bound = _exact_grouped(xe[:off[-1]], off, np.arange(off[-1]), [m[1] for m in pick], x_type, "bf16")
+    _check(got[:off[-1]], exact, bound, "bf16", kind)
+    assert np.all(got[off[-1]:] == 5.0)
+
+
 @pytest.mark.parametrize("x_type,y_type", TYPES[:3])
-@pytest.mark.parametrize("mean", [10, 40])
+@pytest.mark.parametrize("mean,groups", [(10, 130), (10, 260), (40, 130), (40, 260)])
 @pytest.mark.parametrize("kind", sorted(MANY))
-def test_many_groups_swiglu(ctx, oracle, kind, mean, x_type, y_type):
+def test_many_groups_swiglu(ctx, oracle, kind, mean, groups, x_type, y_type):
+    """The same of SwiGLU, with tiles of 128 positions where y is bf16 (40 rows, 260 groups)."""
     from hawking_amd.organs import OrganSet
     from hawking_amd.rows import GroupedSwiGlu, RowGroups
-    say("many groups swiglu", kind, mean, x_type, y_type)
+    say("many groups swiglu", kind, mean, groups, x_type, y_type)
     rows, cols, per_row = 150, MANY[kind], 3
     rng = np.random.default_rng(mean + 1)
-    cs = _many(rng, mean)
+    cs = _many(rng, mean, groups)
     cs += [-sum(cs) % per_row]
     groups, n = len(cs), sum(cs)
     ids = rng.permutation(np.repeat(np.arange(groups), cs)).astype(np.int32)
