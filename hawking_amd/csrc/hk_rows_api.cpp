@@ -72,7 +72,8 @@ constexpr uint32_t TILE8_ROWS = 70, TILE8_ROWS_GLU = 15, TILE8_GROUPS = 2048, TI
 // The int8 engine wants few rows a group.  (The bound on the source rows makes
 // the workspace of a larger batch enough for every smaller one.)
 bool takes_vec(int kind, int form, int wp, uint32_t n, uint32_t groups, uint32_t x_rows, uint32_t cols) {
-    return form != ROWS_LORA && n / std::max(1u, std::min(groups, n)) <= (wp == 2 ? VEC_ROWS : VEC_ROWS_BF16) && x_rows <= (VEC_ROWS + 1u) * groups &&
+    return form != ROWS_LORA && n / std::max(1u, std::min(groups, n)) <= (wp == 2 ? VEC_ROWS : VEC_ROWS_BF16) &&
+           x_rows <= (VEC_ROWS + 1u) * groups &&
            rows_vec_image_bytes(kind, cols) <= VEC_LDS;
 }
 
@@ -106,7 +107,10 @@ RowsShape shape_for(int kind, int form, int32_t x_type, int32_t y_type, uint32_t
     auto groups_of = [&](uint32_t rows) { return (uint64_t)std::max(std::min(groups, n), n / rows) * blocks; };
     sh.tile = groups_of(64) >= (per <= 16 ? TILE_GROUPS_16 : form == ROWS_LORA ? TILE_GROUPS_LORA : TILE_GROUPS_64);
     if (sh.tile)
-        sh.mt = tile8 && per > (form == ROWS_GLU ? TILE8_ROWS_GLU : TILE8_ROWS) && groups_of(128) >= (form == ROWS_GLU ? TILE8_GROUPS_GLU : TILE8_GROUPS) ? 8 : 4;
+        sh.mt = tile8 && per > (form == ROWS_GLU ? TILE8_ROWS_GLU : TILE8_ROWS) &&
+                        groups_of(128) >= (form == ROWS_GLU ? TILE8_GROUPS_GLU : TILE8_GROUPS)
+                    ? 8
+                    : 4;
     else
         sh.mt = per <= 16 ? 1 : 4;
     sh.rt = sh.mt == 4 && (kind == HK_MIXED || groups_of(64) < TILE_RT4_GROUPS) ? 2 : 4;

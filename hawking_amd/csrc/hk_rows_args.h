@@ -47,7 +47,8 @@ inline RowsCheck check_rows(const hk_rows* r, uint32_t cols) {
 inline RowsCheck check_group(const int32_t* ids, uint32_t n, uint32_t groups, const int32_t* offsets, const int32_t* order,
                              const int32_t* pos, const void* ws, size_t ws_bytes, size_t need) {
     if (groups == 0 || groups > 8192) return rows_fail(HK_E_UNSUPPORTED, "n_groups must be in [1, 8192]");
-    if (n > 0x7FFFFFFFu) return rows_fail(HK_E_UNSUPPORTED, "at most 2^31 - 1 ids");
+    // (every part of the ids reads the counts of all parts: the work grows with n^2)
+    if (n > (1u << 24)) return rows_fail(HK_E_UNSUPPORTED, "at most 2^24 ids");
     if (!offsets || (n && (!ids || !order || !pos))) return rows_fail(HK_E_INVALID_ARG, "NULL ids or outputs");
     const size_t b = (size_t)n * 4u, ob = ((size_t)groups + 1u) * 4u;
     if (spans_overlap(ids, b, offsets, ob) || spans_overlap(ids, b, order, b) || spans_overlap(ids, b, pos, b) ||

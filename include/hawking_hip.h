@@ -675,7 +675,7 @@ typedef struct hk_rows {
  * All device int32; ids must not overlap the outputs.  ws: device memory of
  * hk_group_rows_workspace(n, n_groups) bytes (0 up to 8192 ids: ws may be NULL),
  * written by the call.  n may be 0 (offsets are written).  Limits
- * (HK_E_UNSUPPORTED beyond): n < 2^31, 1 <= n_groups <= 8192. */
+ * (HK_E_UNSUPPORTED beyond): n <= 2^24, 1 <= n_groups <= 8192. */
 size_t hk_group_rows_workspace(uint32_t n, uint32_t n_groups);
 int hk_group_rows(hk_ctx* ctx, const int32_t* ids, uint32_t n, uint32_t n_groups, int32_t* offsets, int32_t* order,
                   int32_t* pos, void* ws, size_t ws_bytes, hk_stream stream);

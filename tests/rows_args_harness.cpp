@@ -61,6 +61,7 @@ int main() {
     say("g_no_groups", group(X, 10, 0, O, Y, W, 0, 0, 0));
     say("g_many_groups", group(X, 10, 8193, O, Y, W, 0, 0, 0));
     say("g_many_ids", group(X, 0x80000000u, 4, O, Y, W, 0, 0, 0));
+    say("g_one_id_more", group(X, (1u << 24) + 1u, 4, O, 2 * X + (1u << 28), 3 * X + (1u << 29), 0, 0, 0));
     say("g_null_ids", group(0, 10, 4, O, Y, W, 0, 0, 0));
     say("g_null_pos", group(X, 10, 4, O, Y, 0, 0, 0, 0));
     say("g_null_offsets", group(X, 10, 4, 0, Y, W, 0, 0, 0));

@@ -14,7 +14,8 @@ EXPECT = {
     "y_stride": GEOM, "stride_overflow": GEOM, "too_many": UNSUP, "few_x": GEOM, "no_x": GEOM, "per_row": ARG,
     "null_offsets": ARG, "null_ws": ARG, "misaligned_ws": ARG, "short_ws": ARG, "overlap": ARG, "touching_is_ok": 0,
     "ws_in_x": ARG, "ws_in_y": ARG,
-    "g_ok": 0, "g_ok_empty": 0, "g_no_groups": UNSUP, "g_many_groups": UNSUP, "g_many_ids": UNSUP, "g_null_ids": ARG,
+    "g_ok": 0, "g_ok_empty": 0, "g_no_groups": UNSUP, "g_many_groups": UNSUP, "g_many_ids": UNSUP, "g_one_id_more": UNSUP,
+    "g_null_ids": ARG,
     "g_null_pos": ARG, "g_null_offsets": ARG, "g_alias": ARG, "g_alias_offsets": ARG, "g_no_ws": ARG, "g_short_ws": ARG,
     "c_ok": 0, "c_ok_in_place": 0, "c_ok_no_x": 0, "c_cols": GEOM, "c_per_row": GEOM, "c_null_pos": ARG, "c_null_w": ARG,
     "c_stride": GEOM, "c_base_few": GEOM, "c_base_overlap": ARG, "c_x_overlap": ARG,
